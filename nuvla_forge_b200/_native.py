@@ -15,6 +15,7 @@ is set; ``NUVLA_FORGE_DISABLE_NATIVE=1`` forces the pure-PyTorch reference.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
@@ -89,6 +90,11 @@ _SIGS: dict[str, tuple] = {
     "nfb_is_debug_build": (I, []),
     "nfb_gemm_swiglu_fwd": (I, [P, P, P, P, I, I, I, L, L, L, L, P, P]),
     "nfb_gemm_swiglu_bwd": (I, [P, P, P, P, I, I, I, L, L, L, L, P, P]),
+    "nfb_append_kv": (I, [I, P, P, P, P, P, P, P, P, P, P, P, P, P, P]),
+    "nfb_paged_attn_ws": (L, [L, L, L, L, L]),
+    "nfb_paged_attn": (I, [I, P, P, P, P, P, P, P, P, F, P, P]),
+    "nfb_logprobs_fwd": (I, [I, P, L, L, L, P, L, I, P, P, P, P, P, P, P]),
+    "nfb_logprobs_bwd": (I, [I, P, L, L, L, P, L, I, P, P, P, P, P, P, P, P]),
 }
 
 _lib = None
@@ -212,6 +218,22 @@ def stream(device: torch.device | None = None) -> int:
         idx = device.index if device is not None else None
         return _raw_stream(torch.cuda.current_device() if idx is None else idx)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def int64s(*values: int):
+    """A host array of int64 for entry points that take their sizes and strides as one array."""
+    return (c_int64 * len(values))(*values)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current (kernels launch on the current device)."""
+    idx = device.index
+    if idx is None or idx == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(idx)
 
 
 def dtype_code(dt: torch.dtype) -> int:

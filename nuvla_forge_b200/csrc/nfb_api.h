@@ -230,6 +230,34 @@ NFB_EXPORT int nfb_ag_gemm(const uint64_t* bases, int rank, int world, int64_t s
                            void* stream);
 NFB_EXPORT int nfb_ag_gemm_max_nblocks(void);
 
+/* ---- paged key-value cache: append and attention of one new token (paged.cu) ------------- */
+/* Cache pools [n_pages, page_size, Hkv, D], page ids table [B, table_width] int32. A position or
+ * page id out of range sets the status word (code 3) and is skipped; nothing outside the pools is
+ * touched. q may be null. dims: see paged.cu. */
+NFB_EXPORT int nfb_append_kv(int dtype, const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                             void* v_cache, const int32_t* table, const int32_t* starts, const int32_t* counts,
+                             const float* cos, const float* sin, const int64_t* dims, uint32_t* status,
+                             void* stream);
+/* fp32 values of workspace that nfb_paged_attn needs (capacity = table_width * page_size). */
+NFB_EXPORT int64_t nfb_paged_attn_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity);
+NFB_EXPORT int nfb_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* table, const int32_t* lengths, void* out, float* ws,
+                              const int64_t* dims, float scale, uint32_t* status, void* stream);
+
+/* ---- token log probabilities, entropy and top alternatives (logprobs.cu) ----------------- */
+/* stats receives (max, sum of exp(z - max)) per row for the backward pass; targets may be null. A
+ * target outside [0, V) other than ignore_index gives NaN and sets the status word (code 3).
+ * top_k <= 32. */
+NFB_EXPORT int nfb_logprobs_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V,
+                                const int64_t* targets, int64_t ignore_index, int top_k, float* logprobs,
+                                float* entropy, float* stats, float* top_logprobs, int64_t* top_tokens,
+                                uint32_t* status, void* stream);
+/* Null g_* pointers: no gradient from that output. */
+NFB_EXPORT int nfb_logprobs_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V,
+                                const int64_t* targets, int64_t ignore_index, int top_k, const int64_t* top_tokens,
+                                const float* g_logprobs, const float* g_entropy, const float* g_top,
+                                const float* stats, const float* entropy, void* d_logits, void* stream);
+
 /* ---- host-side synthetic data (synth.cpp) ----------------------------------------------- */
 /* Fills n bytes with a counter-based pseudo-random stream of (seed, index) using `threads`
  * host threads (the same bytes for any thread count). */

@@ -31,10 +31,11 @@ class DeviceFault(RuntimeError):
 
 def status_words(model=None) -> list[tuple[str, torch.Tensor]]:
     """Every device status word the native ops and the parallel runtime have created so far."""
-    from .ops import ce_tc, flash_attn, linear, norm
+    from .ops import ce_tc, flash_attn, linear, logprobs, norm, paged
 
     out = []
-    for name, mod in (("gemm", linear), ("cross_entropy", ce_tc), ("norm", norm), ("attention", flash_attn)):
+    for name, mod in (("gemm", linear), ("cross_entropy", ce_tc), ("norm", norm), ("attention", flash_attn),
+                      ("paged_cache", paged), ("logprobs", logprobs)):
         for idx, t in sorted(getattr(mod, "_status", {}).items()):
             out.append((f"{name}@cuda:{idx}", t))
     ws = getattr(model, "ws", None)

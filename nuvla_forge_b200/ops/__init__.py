@@ -10,18 +10,24 @@ from . import flash_attn  # noqa: F401  (tcgen05 attention forward; opt-in via N
 from .attention import attention
 from .chunked_ce import chunked_cross_entropy
 from .image import normalise_images, patchify_images
+from .logprobs import TokenLogprobs, token_logprobs
 from .norm import add_rmsnorm, fused_adaln_residual_rmsnorm, rmsnorm
+from .paged import append_kv, paged_attention
 from .swiglu import fused_swiglu, swiglu_packed
 
 __all__ = [
     "HAS_NATIVE",
+    "TokenLogprobs",
     "add_rmsnorm",
+    "append_kv",
     "attention",
     "chunked_cross_entropy",
     "fused_adaln_residual_rmsnorm",
     "fused_swiglu",
     "normalise_images",
+    "paged_attention",
     "patchify_images",
     "rmsnorm",
     "swiglu_packed",
+    "token_logprobs",
 ]

@@ -1,0 +1,134 @@
+"""Log probabilities of given tokens, entropy and the most likely tokens (native csrc/logprobs.cu).
+
+``token_logprobs`` reads materialised logits once and returns what scoring, serving and fine-tuning
+on scores need; unlike ``chunked_cross_entropy``, which keeps only a mean loss, it keeps each token's
+value and is differentiable in all of them. Sums are fp32 whatever the logits' type; the gradient is
+computed in fp32 and rounded once to it.
+
+The reference project has only the mean cross entropy.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _native as nat
+from .reference import token_logprobs_ref
+
+MAX_TOP_K = 32
+
+_status: dict[int, torch.Tensor] = {}
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor | None       # [...] fp32 log p of the targets (0 where ignored)
+    entropy: torch.Tensor               # [...] fp32, in nats
+    top_logprobs: torch.Tensor | None   # [..., top_k] fp32, descending
+    top_tokens: torch.Tensor | None     # [..., top_k] int64
+
+
+def _status_word(device: torch.device) -> torch.Tensor:
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    t = _status.get(idx)
+    if t is None:
+        t = _status[idx] = torch.zeros(1, dtype=torch.int32, device=device)
+    return t
+
+
+def check_status(device: torch.device | None = None) -> None:
+    """Raise if a kernel met a target outside the vocabulary (synchronises)."""
+    for idx, t in _status.items():
+        v = int(t.item())
+        if v:
+            t.zero_()
+            raise RuntimeError(f"token_logprobs on cuda:{idx}: a target is outside the vocabulary (status {v:#x})")
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, targets, top_k, ignore_index):
+        M, V = x.shape
+        dev = x.device
+        f32 = dict(dtype=torch.float32, device=dev)
+        logprobs = torch.empty(M, **f32) if targets is not None else None
+        entropy = torch.empty(M, **f32)
+        stats = torch.empty((M, 2), **f32)
+        top = torch.empty((M, top_k), **f32) if top_k else None
+        ids = torch.empty((M, top_k), dtype=torch.int64, device=dev) if top_k else None
+        with nat.on_device(dev):
+            nat.call("nfb_logprobs_fwd", nat.DT[x.dtype], x.data_ptr(), x.stride(0), M, V, nat.ptr(targets),
+                     ignore_index, top_k, nat.ptr(logprobs), entropy.data_ptr(), stats.data_ptr(), nat.ptr(top),
+                     nat.ptr(ids), _status_word(dev).data_ptr(), nat.stream(dev))
+        if ctx is not None:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(x, targets, stats, entropy, ids)
+            ctx.top_k, ctx.ignore_index = top_k, ignore_index
+            if ids is not None:
+                ctx.mark_non_differentiable(ids)
+        return logprobs, entropy, top, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logprobs, g_entropy, g_top, _):
+        x, targets, stats, entropy, ids = ctx.saved_tensors
+        if g_logprobs is None and g_entropy is None and g_top is None:
+            return None, None, None, None
+        M, V = x.shape
+        g_logprobs, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logprobs, g_entropy, g_top))
+        dx = torch.empty((M, V), dtype=x.dtype, device=x.device)
+        with nat.on_device(x.device):
+            nat.call("nfb_logprobs_bwd", nat.DT[x.dtype], x.data_ptr(), x.stride(0), M, V, nat.ptr(targets),
+                     ctx.ignore_index, ctx.top_k, nat.ptr(ids), nat.ptr(g_logprobs), nat.ptr(g_entropy),
+                     nat.ptr(g_top), stats.data_ptr(), entropy.data_ptr(), dx.data_ptr(), nat.stream(x.device))
+        return dx, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top_k: int = 0,
+                   ignore_index: int = -100, force_reference: bool = False) -> TokenLogprobs:
+    """log p of ``targets`` [...] int64 under ``logits`` [..., V], the entropy of each row and its ``top_k``
+    (at most 32) most likely tokens, equal logits in the order of their index.
+
+    Gradients flow from ``logprobs``, ``entropy`` and ``top_logprobs`` to ``logits``. A target equal to
+    ``ignore_index`` has log p 0 and no gradient; its row's entropy and alternatives are computed all the
+    same. A masked logit is -inf; a row of nothing else has log p -inf, entropy 0 and no gradient. A row
+    with a NaN or +inf logit gives NaN (and unspecified alternatives). A target outside the vocabulary
+    gives NaN and is reported by ``check_status`` (on the CPU it raises).
+    """
+    if logits.dim() < 1 or not logits.is_floating_point():
+        raise TypeError(f"logits must be a floating-point tensor [..., V], got {tuple(logits.shape)} {logits.dtype}")
+    V = logits.shape[-1]
+    lead = logits.shape[:-1]
+    if not 0 <= top_k <= min(MAX_TOP_K, V):
+        raise ValueError(f"top_k {top_k} is not in 0..{min(MAX_TOP_K, V)}")
+    if V < 1:
+        raise ValueError("the vocabulary is empty")
+    if targets is not None:
+        if targets.dtype != torch.int64:
+            raise TypeError(f"targets must be int64, got {targets.dtype}")
+        if targets.shape != lead or targets.device != logits.device:
+            raise ValueError(f"targets must be {tuple(lead)} on {logits.device}, got {tuple(targets.shape)} on "
+                             f"{targets.device}")
+    top_k, ignore_index = int(top_k), int(ignore_index)
+    x = logits.reshape(-1, V)
+    t = None if targets is None else targets.reshape(-1)
+    if force_reference or not (nat.HAS_NATIVE and x.is_cuda and x.dtype in nat.DT):
+        r = token_logprobs_ref(x, t, top_k, ignore_index)
+    else:
+        if x.stride(1) != 1 and V > 1:
+            x = x.contiguous()
+        t = None if t is None else t.contiguous()
+        if x.requires_grad and torch.is_grad_enabled():
+            r = _TokenLogprobs.apply(x, t, top_k, ignore_index)
+        else:
+            r = _TokenLogprobs.forward(None, x, t, top_k, ignore_index)
+    if len(lead) == 1:
+        return TokenLogprobs(*r)
+    lp, h, top, ids = r
+    return TokenLogprobs(None if lp is None else lp.view(lead), h.view(lead),
+                         None if top is None else top.view(*lead, top_k), None if ids is None else ids.view(*lead, top_k))
+
+
+__all__ = ["MAX_TOP_K", "TokenLogprobs", "check_status", "token_logprobs"]

@@ -1,0 +1,192 @@
+"""Paged key-value cache: append with position rotation, and attention of one new token (native csrc/paged.cu).
+
+``append_kv`` stores new keys and values where a page table says, rotating the keys (and the
+queries, when given) by their position on the way; ``paged_attention`` attends one query per
+sequence over its cached tokens. Together they are one decoding step of the backbone; the prompt
+enters the cache with the same ``append_kv`` while ``ops.attention`` computes its outputs.
+
+Layout: pools ``[n_pages, page_size, Hkv, D]`` for keys and values (the projection-native order of
+``ops.attention``), ``page_table`` [B, W] int32 page ids, ``lengths`` [B] int32. Token p of sequence
+b is in page ``page_table[b, p // page_size]``, slot ``p % page_size``; any page size works. Lengths
+and page ids stay on the device: neither op waits for the host, both can be captured in a CUDA
+graph, and several streams can run them at once on caches of their own.
+
+A position or page id out of range cannot be refused without reading it back: the kernels skip the
+token and set a status word that ``check_status`` (and the trainer's health monitor) raises on. On
+the CPU the reference raises IndexError. Neither op has a backward pass.
+
+The reference project has no decoding path.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _native as nat
+from .reference import append_kv_ref, paged_attention_ref
+
+MAX_HEAD_DIM = 256
+
+_status: dict[int, torch.Tensor] = {}
+_ws_floats: dict[tuple, int] = {}
+
+
+def _status_word(device: torch.device) -> torch.Tensor:
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    t = _status.get(idx)
+    if t is None:
+        t = _status[idx] = torch.zeros(1, dtype=torch.int32, device=device)
+    return t
+
+
+def check_status(device: torch.device | None = None) -> None:
+    """Raise if a kernel met a position, length or page id out of range (synchronises)."""
+    for idx, t in _status.items():
+        v = int(t.item())
+        if v:
+            t.zero_()
+            raise RuntimeError(f"paged cache on cuda:{idx}: a position, length or page id is out of range "
+                               f"(status {v:#x}, site {v & 0xFFFFFF})")
+
+
+def _check_cache(k_cache, v_cache, page_table, lengths, like, heads: int, dim: int, batch: int) -> None:
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache and v_cache must both be [n_pages, page_size, Hkv, D], got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if k_cache.shape[1] < 1 or k_cache.shape[2] != heads or k_cache.shape[3] != dim:
+        raise ValueError(f"cache {tuple(k_cache.shape)} does not hold {heads} heads of {dim}")
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("the cache's last dimension must be contiguous")
+    if k_cache.dtype != like.dtype or v_cache.dtype != like.dtype:
+        raise TypeError(f"cache dtypes {k_cache.dtype} and {v_cache.dtype} differ from the tokens' {like.dtype}")
+    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise TypeError("page_table and lengths must be int32")
+    if page_table.dim() != 2 or page_table.shape[0] != batch or lengths.shape != (batch,):
+        raise ValueError(f"page_table must be [{batch}, W] and lengths [{batch}], got {tuple(page_table.shape)} "
+                         f"and {tuple(lengths.shape)}")
+    dev = like.device
+    if not (k_cache.device == v_cache.device == page_table.device == lengths.device == dev):
+        raise ValueError("all tensors must be on one device")
+
+
+def _check_no_grad(op: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op} has no backward pass: call it under torch.no_grad()")
+
+
+def _inner(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None,
+              q: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+              interleaved: bool = False, force_reference: bool = False) -> torch.Tensor | None:
+    """Store tokens k, v [B, T, Hkv, D] behind each sequence's ``lengths[b]`` cached tokens, in place.
+
+    Token t of sequence b goes to position ``lengths[b] + t``; with ``counts`` [B] int32 only the
+    first ``counts[b]`` of its T tokens are stored (a padded batch; 0 leaves the sequence as it is).
+    With ``cos`` and ``sin`` ([positions, half] fp32, row p for position p) the first ``2 * half``
+    values of each key head, and of each head of ``q`` [B, T, Hq, D], are rotated: value i with
+    value half + i, or with ``interleaved`` neighbours (2i, 2i + 1); in fp32, rounded once.
+
+    Returns q rotated (a new tensor; padding rows too, at most by the tables' last row), a copy of q
+    without tables, or None without q. ``lengths`` is not changed. The slots that one call writes
+    must be distinct.
+    """
+    if k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"k and v must both be [B, T, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
+    B, T, Hkv, D = k.shape
+    _check_cache(k_cache, v_cache, page_table, lengths, k, Hkv, D, B)
+    if v.dtype != k.dtype or v.device != k.device:
+        raise TypeError("k and v must share dtype and device")
+    if q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != D or q.dtype != k.dtype
+                          or q.device != k.device):
+        raise ValueError(f"q must be [{B}, {T}, Hq, {D}] of {k.dtype} on {k.device}, got {tuple(q.shape)} {q.dtype}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin must be given together")
+    half = 0
+    if cos is not None:
+        half = cos.shape[-1]
+        if cos.dim() != 2 or cos.shape != sin.shape or not 0 < 2 * half <= D or cos.shape[0] < 1:
+            raise ValueError(f"cos and sin must be [positions, half] with 2 * half <= {D}, got {tuple(cos.shape)} "
+                             f"and {tuple(sin.shape)}")
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != k.device or sin.device != k.device:
+            raise TypeError("cos and sin must be fp32 on the tokens' device")
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,) or counts.device != k.device):
+        raise TypeError(f"counts must be [{B}] int32 on {k.device}")
+    if any(n > 1 and s == 0 for c in (k_cache, v_cache) for n, s in zip(c.shape, c.stride())):
+        raise ValueError("the cache must not be an expanded tensor: its slots would share memory")
+    _check_no_grad("append_kv", k, v, q, k_cache, v_cache)
+    if force_reference or not (nat.HAS_NATIVE and k.is_cuda and k.dtype in nat.DT):
+        out = append_kv_ref(k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
+        return out.clone() if out is q and q is not None else out
+    k, v = _inner(k), _inner(v)
+    page_table, lengths = _inner(page_table), lengths.contiguous()
+    out = None
+    Hq, qs = 0, (0, 0, 0)
+    if q is not None:
+        q = _inner(q)
+        Hq, qs = q.shape[2], q.stride()[:3]
+        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    rope_rows = 0
+    if half:
+        cos, sin = cos.contiguous(), sin.contiguous()
+        rope_rows = cos.shape[0]
+    if counts is not None:
+        counts = counts.contiguous()
+    dims = nat.int64s(B, T, Hq, Hkv, D, half, int(interleaved), k_cache.shape[1], k_cache.shape[0],
+                      page_table.shape[1], rope_rows, *qs, *k.stride()[:3], *v.stride()[:3],
+                      *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0))
+    with nat.on_device(k.device):
+        nat.call("nfb_append_kv", nat.DT[k.dtype], nat.ptr(q), k.data_ptr(), v.data_ptr(), nat.ptr(out),
+                 k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+                 nat.ptr(counts), nat.ptr(cos), nat.ptr(sin), dims, _status_word(k.device).data_ptr(),
+                 nat.stream(k.device))
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, scale: float | None = None,
+                    force_reference: bool = False) -> torch.Tensor:
+    """softmax(scale q k^T) v of one query per sequence over its first ``lengths[b]`` cached tokens.
+
+    q [B, 1, Hq, D] (grouped queries: Hkv divides Hq, D <= 256); returns [B, 1, Hq, D]. ``scale``
+    defaults to D ** -0.5. A sequence of length 0 answers zeros; what the pages hold behind a
+    sequence's length is never used. Statistics and sums are fp32, whatever the cache's type.
+    """
+    if q.dim() != 4 or q.shape[1] != 1:
+        raise ValueError(f"q must be [B, 1, Hq, D], got {tuple(q.shape)}")
+    B, _, Hq, D = q.shape
+    Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
+    _check_cache(k_cache, v_cache, page_table, lengths, q, Hkv, D, B)
+    if Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hkv} key heads do not divide {Hq} query heads")
+    if not 0 < D <= MAX_HEAD_DIM:
+        raise ValueError(f"head size {D} is not in 1..{MAX_HEAD_DIM}")
+    _check_no_grad("paged_attention", q, k_cache, v_cache)
+    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    if force_reference or not (nat.HAS_NATIVE and q.is_cuda and q.dtype in nat.DT):
+        return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, sc)
+    q = _inner(q)
+    page_table, lengths = _inner(page_table), lengths.contiguous()
+    n_pages, ps = k_cache.shape[:2]
+    W = page_table.shape[1]
+    out = torch.empty((B, 1, Hq, D), dtype=q.dtype, device=q.device)
+    key = (B, Hq, Hkv, D, ps * W)
+    n = _ws_floats.get(key)
+    if n is None:
+        n = _ws_floats[key] = int(nat.lib().nfb_paged_attn_ws(*key))
+    ws = torch.empty(n, dtype=torch.float32, device=q.device)
+    dims = nat.int64s(B, Hq, Hkv, D, ps, n_pages, W, q.stride(0), q.stride(2), Hq * D, D, *k_cache.stride()[:3],
+                      *v_cache.stride()[:3], page_table.stride(0))
+    with nat.on_device(q.device):
+        nat.call("nfb_paged_attn", nat.DT[q.dtype], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                 page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), ws.data_ptr(), dims, sc,
+                 _status_word(q.device).data_ptr(), nat.stream(q.device))
+    return out
+
+
+__all__ = ["MAX_HEAD_DIM", "append_kv", "check_status", "paged_attention"]

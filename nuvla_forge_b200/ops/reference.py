@@ -79,6 +79,93 @@ def attention_ref(q, k, v, causal: bool = False, scale: float | None = None):
     return torch.einsum("bhsl,bhld->bhsd", p, vf).to(q.dtype)
 
 
+def _cache_slots(page_table, positions, n_pages: int, page_size: int):
+    """(page, slot) of each position [B, T]; raises on a position or page id out of range."""
+    if positions.numel() and (int(positions.min()) < 0 or int(positions.max()) >= page_table.shape[1] * page_size):
+        raise IndexError("a position lies outside the pages of its sequence")
+    page = page_table.long().gather(1, positions // page_size)
+    if page.numel() and (int(page.min()) < 0 or int(page.max()) >= n_pages):
+        raise IndexError("a page id lies outside the cache")
+    return page, positions % page_size
+
+
+def rotate_ref(x, cos, sin, interleaved: bool = False):
+    """Rotates the first 2 * half values of each head of x [B, T, H, D] by cos / sin [B, T, half], in fp32."""
+    half = cos.shape[-1]
+    xf = x.to(torch.float32)
+    c, s = cos[:, :, None], sin[:, :, None]
+    if interleaved:
+        a, b = xf[..., 0:2 * half:2], xf[..., 1:2 * half:2]
+        turned = torch.stack([a * c - b * s, b * c + a * s], dim=-1).flatten(-2)
+    else:
+        a, b = xf[..., :half], xf[..., half:2 * half]
+        turned = torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+    return torch.cat([turned.to(x.dtype), x[..., 2 * half:]], dim=-1)
+
+
+def append_kv_ref(k, v, k_cache, v_cache, page_table, lengths, counts=None, q=None, cos=None, sin=None,
+                  interleaved: bool = False):
+    """Stores the rotated keys and the values of tokens t < counts[b] at positions lengths[b] + t; returns rotated q."""
+    B, T = k.shape[:2]
+    t = torch.arange(T, device=k.device)
+    pos = lengths.long()[:, None] + t
+    live = t < counts[:, None] if counts is not None else torch.ones_like(pos, dtype=torch.bool)
+    if cos is not None:
+        if bool(((pos < 0) | (pos >= cos.shape[0]))[live].any()):
+            raise IndexError("a position lies outside the cos / sin tables")
+        at = pos.clamp(0, max(cos.shape[0] - 1, 0))
+        k = rotate_ref(k, cos[at], sin[at], interleaved)
+        q = rotate_ref(q, cos[at], sin[at], interleaved) if q is not None else None
+    rows = torch.arange(B, device=k.device)[:, None].expand(B, T)[live]
+    page, slot = _cache_slots(page_table[rows], pos[live][:, None], k_cache.shape[0], k_cache.shape[1])
+    k_cache[page[:, 0], slot[:, 0]] = k[live]
+    v_cache[page[:, 0], slot[:, 0]] = v[live]
+    return q
+
+
+def paged_attention_ref(q, k_cache, v_cache, page_table, lengths, scale: float | None = None):
+    """Softmax attention in fp32 of q [B, 1, Hq, D] over each sequence's first lengths[b] cached tokens."""
+    B, _, hq, d = q.shape
+    n_pages, ps, hkv, _ = k_cache.shape
+    out = torch.zeros((B, 1, hq, d), dtype=q.dtype, device=q.device)
+    for b, n in enumerate(lengths.tolist()):
+        if n < 0:
+            raise IndexError("a length is negative")
+        if n == 0:
+            continue
+        page, slot = _cache_slots(page_table[b:b + 1], torch.arange(n, device=q.device)[None], n_pages, ps)
+        # attention_ref leaves a row of -inf scores as NaN; a query no key is left for answers 0
+        k, v = (c[page, slot].transpose(1, 2) for c in (k_cache, v_cache))
+        o = attention_ref(q[b:b + 1].transpose(1, 2), k, v, scale=scale)
+        kf = k.to(torch.float32).repeat_interleave(hq // hkv, dim=1)
+        sc = scale if scale is not None else 1.0 / math.sqrt(d)
+        s = torch.einsum("bhsd,bhld->bhsl", q[b:b + 1].transpose(1, 2).to(torch.float32), kf) * sc
+        o = torch.where((s == float("-inf")).all(dim=-1, keepdim=True), torch.zeros_like(o), o)
+        out[b:b + 1] = o.transpose(1, 2)
+    return out
+
+
+def token_logprobs_ref(logits, targets=None, top_k: int = 0, ignore_index: int = -100):
+    """(log p of the targets or None, entropy, top log p or None, top ids or None) of logits [M, V], in fp32
+    (fp64 logits: in fp64). A row without a finite logit: log p -inf, entropy 0, no gradient."""
+    x = logits if logits.dtype == torch.float64 else logits.to(torch.float32)
+    dead = (x == float("-inf")).all(dim=-1, keepdim=True)
+    logp = torch.log_softmax(torch.where(dead, torch.zeros_like(x), x), dim=-1)
+    p = logp.exp()
+    entropy = -(p * torch.where(p > 0, logp, torch.zeros_like(logp))).sum(dim=-1)
+    entropy = torch.where(dead[:, 0], torch.zeros_like(entropy), entropy)
+    none = torch.full((), float("-inf"), dtype=x.dtype, device=x.device)
+    given = top = ids = None
+    if targets is not None:
+        keep = targets != ignore_index
+        lp = logp.gather(1, torch.where(keep, targets, torch.zeros_like(targets))[:, None])
+        given = torch.where(keep, torch.where(dead, none, lp)[:, 0], torch.zeros_like(entropy))
+    if top_k:
+        ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True)[1][:, :top_k].contiguous()
+        top = torch.where(dead, none, logp.gather(1, ids))
+    return given, entropy, top, ids
+
+
 def normalise_images_ref(images, dtype=torch.bfloat16, mean=IMAGENET_MEAN, std=IMAGENET_STD):
     """uint8 [..., 3, H, W] -> (v/255 - mean[c]) / std[c] in ``dtype``."""
     x = images.to(torch.float32) / 255.0
