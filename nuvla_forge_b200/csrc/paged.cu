@@ -187,6 +187,7 @@ struct AttnArgs {
   uint32_t* status;
   int B, Hq, Hkv, D, G;        // G = Hq / Hkv query heads per key head
   int rows, subs, units;       // query heads a unit covers; units per key head; units per sequence
+  int whole;                   // one CTA for each (sequence, unit): nothing is shared
   int ctas, min_tiles;
   int page_size, n_pages, table_width;
   int64_t q_sb, q_sh, o_sb, o_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, t_sb;
@@ -213,78 +214,114 @@ __device__ __forceinline__ int64_t warp_incl_scan(int64_t v) {
   return v;
 }
 
-// Tiles of all sequences before `upto` (warp-collective).
-__device__ __forceinline__ int64_t tiles_before(const AttnArgs& a, int upto) {
-  int64_t n = 0;
-  for (int b = threadIdx.x & 31; b < upto; b += 32) n += seq_tiles(a, b);
+// Tiles of the sequences before `upto`, and of all (warp-collective).
+__device__ __forceinline__ void tiles_before_and_all(const AttnArgs& a, int upto, int64_t& before, int64_t& all) {
+  before = all = 0;
+#pragma unroll 4
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+    const int t = seq_tiles(a, b);
+    all += t;
+    if (b < upto) before += t;
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
 }
 
 __device__ __forceinline__ int64_t tiles_per_cta(const AttnArgs& a, int64_t all) {
   const int64_t total = all * a.units;
-  return max((int64_t)a.min_tiles, (total + a.ctas - 1) / a.ctas);
+  // (a 64-bit division costs ten times the 32-bit one)
+  const int64_t even = total < INT_MAX - a.ctas ? (int)((uint32_t)(total + a.ctas - 1) / (uint32_t)a.ctas)
+                                                : (total + a.ctas - 1) / a.ctas;
+  return max((int64_t)a.min_tiles, even);
 }
 
-// The sequence that holds list position pos, and the tiles before it (warp-collective).
-__device__ __forceinline__ void find_seq(const AttnArgs& a, int64_t pos, int& b, int64_t& before) {
-  int64_t done = 0;
+// All tiles, and the sequence that holds list position cta * per with the tiles before it (b = B
+// where the list has no such position). Warp-collective; the lengths of up to 128 sequences are read
+// once, of more twice.
+__device__ __forceinline__ void find_start(const AttnArgs& a, int64_t cta, int64_t& total, int64_t& per, int& b,
+                                           int64_t& before) {
+  constexpr int kHeld = 4;
   const int lane = threadIdx.x & 31;
+  int held[kHeld];
+  int64_t all = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < a.B ? seq_tiles(a, 32 * i + lane) : 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) all += held[i];
+  for (int s = 32 * kHeld + lane; s < a.B; s += 32) all += seq_tiles(a, s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  total = all * a.units;
+  per = tiles_per_cta(a, all);
+  const int64_t pos = cta * per;
   b = a.B;
   before = 0;
+  if (pos >= total) return;
+  int64_t done = 0;
   for (int base = 0; base < a.B; base += 32) {
-    const int64_t t = base + lane < a.B ? seq_tiles(a, base + lane) : 0;
-    const int64_t incl = done + warp_incl_scan(t);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) mine = base == 32 * i ? held[i] : mine;
+    if (base >= 32 * kHeld) mine = base + lane < a.B ? seq_tiles(a, base + lane) : 0;
+    const int64_t incl = done + warp_incl_scan(mine);
     const uint32_t hit = __ballot_sync(0xffffffffu, pos < incl * a.units);
     if (hit) {
-      const int l = __ffs(hit) - 1;
-      b = base + l;
-      before = __shfl_sync(0xffffffffu, incl - t, l);
+      const int s = __ffs(hit) - 1;
+      b = base + s;
+      before = __shfl_sync(0xffffffffu, incl - mine, s);
       return;
     }
     done = __shfl_sync(0xffffffffu, incl, 31);
   }
 }
 
-// One CTA's part of one (sequence, unit).
-struct Part {
+// A CTA's run of the list, one (sequence, unit) at a time: the fields describe the current part.
+struct Parts {
   int b, kvh, row0, rows;  // sequence, key head, first query head and number of query heads
   int tile0, tile1, len;
-  int slot;                // workspace slot, or -1: the CTA covers all of it and finishes the rows
-};
+  int slot;                // workspace slot, or -1: the CTA covers all of the unit and finishes its rows
+  int unit, tiles;
+  int64_t left;            // tiles of the run behind this part
 
-// Walks the CTA's run of the list.
-template <typename F>
-__device__ __forceinline__ void for_each_part(const AttnArgs& a, F&& f) {
-  const int64_t total = tiles_before(a, a.B) * a.units;
-  const int64_t per = tiles_per_cta(a, total / a.units);
-  int64_t pos = (int64_t)blockIdx.x * per;
-  const int64_t end = min(pos + per, total);
-  if (pos >= end) return;
-  const int64_t first = pos;
-  int b;
-  int64_t before;
-  find_seq(a, pos, b, before);
-  int len = seq_len(a, b), tiles = (len + kTile - 1) / kTile;
-  const int64_t off = pos - before * a.units;
-  int unit = (int)(off / tiles), tile = (int)(off - (int64_t)unit * tiles);
-  while (true) {
-    const int n = (int)min((int64_t)(tiles - tile), end - pos);
-    Part p;
-    p.b = b;
-    p.kvh = unit / a.subs;
-    const int sub = unit - p.kvh * a.subs;
-    p.row0 = p.kvh * a.G + sub * a.rows;
-    p.rows = min(a.rows, a.G - sub * a.rows);
-    p.tile0 = tile;
-    p.tile1 = tile + n;
-    p.len = len;
-    p.slot = n == tiles ? -1 : (int)(2 * blockIdx.x + (pos == first ? 0 : 1));
-    f(p);
-    pos += n;
-    if (pos >= end) break;
-    tile = 0;
+  __device__ __forceinline__ void set(const AttnArgs& a, int tile, int free_slot) {
+    kvh = unit / a.subs;
+    const int sub = unit - kvh * a.subs;
+    row0 = kvh * a.G + sub * a.rows;
+    rows = min(a.rows, a.G - sub * a.rows);
+    const int n = (int)min((int64_t)(tiles - tile), left);
+    tile0 = tile;
+    tile1 = tile + n;
+    left -= n;
+    slot = n == tiles ? -1 : free_slot;
+  }
+  // False: the CTA has nothing to do. (All warps of the CTA compute the same.)
+  __device__ __forceinline__ bool first(const AttnArgs& a) {
+    if (a.whole) {
+      b = blockIdx.x / a.units;
+      unit = blockIdx.x - b * a.units;
+      len = seq_len(a, b);
+      tiles = (len + kTile - 1) / kTile;
+      left = tiles;
+      set(a, 0, -1);
+      return len > 0;
+    }
+    int64_t total, per, before;
+    find_start(a, blockIdx.x, total, per, b, before);
+    if (b == a.B) return false;
+    const int64_t pos = (int64_t)blockIdx.x * per;
+    left = min(per, total - pos);
+    len = seq_len(a, b);
+    tiles = (len + kTile - 1) / kTile;
+    const int64_t off = pos - before * a.units;
+    unit = off <= INT_MAX ? (int)((uint32_t)off / (uint32_t)tiles) : (int)(off / tiles);
+    set(a, (int)(off - (int64_t)unit * tiles), 2 * blockIdx.x);
+    return true;
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& a) {
+    if (left == 0) return false;
     if (++unit == a.units) {
       unit = 0;
       do {
@@ -292,6 +329,20 @@ __device__ __forceinline__ void for_each_part(const AttnArgs& a, F&& f) {
         len = seq_len(a, b);
       } while (len == 0);
       tiles = (len + kTile - 1) / kTile;
+    }
+    set(a, 0, 2 * blockIdx.x + 1);
+    return true;
+  }
+};
+
+// Rows of zeros for the empty sequences, dealt out over the CTAs.
+template <typename T>
+__device__ __forceinline__ void zero_empty(const AttnArgs& a) {
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (seq_len(a, b) != 0) continue;
+    for (int i = threadIdx.x; i < a.Hq * a.D; i += blockDim.x) {
+      const int h = i / a.D;
+      ((T*)a.out)[b * a.o_sb + h * a.o_sh + (i - h * a.D)] = from_f32<T>(0.f);
     }
   }
 }
@@ -306,8 +357,10 @@ template <typename T, int DP, int GC>
 __global__ void __launch_bounds__(32 * kAttnWarps) attn_plain_kernel(const AttnArgs a) {
   __shared__ float s_o[kAttnWarps][GC][32 * DP];
   __shared__ float s_m[kAttnWarps][GC], s_l[kAttnWarps][GC];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for_each_part(a, [&](const Part& p) {
+  Parts p;
+  for (bool more = p.first(a); more; more = p.next(a)) {
     float q[GC][DP], o[GC][DP], m[GC], l[GC];
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
@@ -414,40 +467,486 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_plain_kernel(const AttnA
       }
     }
     __syncthreads();
-  });
+  }
+  zero_empty<T>(a);
 }
 
-// Combines the parts of each (sequence, query head) that several CTAs share, in list order, and
-// writes the zero rows of empty sequences. One block per sequence and query head.
-template <typename T>
+// Tensor-core kernel for 16-bit caches. A warp takes tiles of 16 tokens and multiplies them with
+// mma.m16n8k16, the tokens and values on the 16-row side and 8 query heads on the 8-column side:
+//   S^T = K Q^T    (16 tokens x 8 heads x 16 values a step),
+//   O^T += V^T P^T (16 values x 8 heads x 16 tokens a step).
+// The work is bound by the cache's bytes (2 Hq / Hkv products for each value read), so the small
+// warp-level shape is the right one: the 128 rows of a tcgen05 tile would stay empty.
+//
+// K: the product does not care which value a k index stands for, so a lane's 16-byte piece of a key
+// row (values 8j.. of each 32) is the A fragment of two steps, with Q held in the same order. V is
+// read transposed by ldmatrix. Weights leave the S^T fragments for the P^T ones by an 8 x 8 transpose
+// in registers, and each head's maximum and sum live in the lanes that hold its columns of O^T.
+//
+// The weights p = exp(z - m) would lose 8 bits (bf16) as an operand, so they go in as two: hi, p
+// rounded a little low so that p - hi > 0, and the rest; one step is two products, 2^-16 of p is left
+// (fp16: 2^-20), and an infinite value stays infinite because both parts are positive. Sums of
+// weights use the fp32 values. The running maximum moves only when a score passes it by more than
+// 2^8: the sums have the room, and the rescaling, with its exchange between lanes, becomes rare.
+template <typename T> struct Mma;
+template <> struct Mma<__nv_bfloat16> {
+  static constexpr float kLow = 1.f - 0x1p-8f;
+  static __device__ __forceinline__ void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  }
+};
+template <> struct Mma<__half> {
+  static constexpr float kLow = 1.f - 0x1p-10f;
+  static __device__ __forceinline__ void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+};
+
+// Asynchronous copies of 16 bytes to shared memory; off: nothing is read and zeros are stored.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ldmatrix4t(uint32_t p) {
+  uint4 v;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Shared-memory layout of a tile: 16 rows of keys, then 16 of values, kPitch bytes each; the 16-byte
+// pieces of a row are permuted by the row so that the fragment reads (two key rows by four pieces,
+// eight value rows by one piece at a time) touch every bank once.
+template <int D> struct Tile {
+  static constexpr int kPieces = D / 8;                              // 16-byte pieces of a row
+  static constexpr int kPitch = D == 32 ? 64 : D == 64 ? 128 : 256;  // D = 96: padded, the permutation needs it
+  static constexpr int kV = kTile * kPitch, kStage = 2 * kV;
+  static constexpr int kCopies = kTile * kPieces / 32;               // copies a lane makes for each of K and V
+  static __device__ __forceinline__ int k_at(int t, int piece) {
+    return t * kPitch + ((D == 32 ? piece : piece ^ ((t & 1) << 2)) << 4);
+  }
+  static __device__ __forceinline__ int v_at(int t, int piece) {
+    return kV + t * kPitch + ((D == 32 ? piece ^ (t >> 1 & 3) : piece ^ (t & 7)) << 4);
+  }
+};
+// Tiles in each warp's ring.
+template <int D> constexpr int ring_stages() { return D <= 64 ? 4 : 2; }
+template <int D> constexpr int attn_smem() {
+  return kAttnWarps * (ring_stages<D>() * Tile<D>::kStage + 4 * (D + 4) * 4) + 256;
+}
+
+// The fetching side of a warp: it walks the run on its own, the ring's depth ahead of the products and
+// across the borders of parts.
+template <typename T, int D, bool PAGE16>
+struct TileFetch {
+  using L = Tile<D>;
+  static constexpr int S = ring_stages<D>();
+  const AttnArgs& a;
+  const int lane, warp;
+  Parts p;
+  bool more;        // p is a part with tiles left to fetch
+  int next;         // next tile of it
+  const T *kb, *vb; // the part's key head in page 0
+  // where the tiles are: PAGE16: lane i has (page, slot) of tile first + 4 i, `have` of them left; else
+  // lane i < 16 of token i of the next tile. page -1: not to be read.
+  int pg, sl, have;
+  uint64_t masks;   // live tokens of the tiles in the ring, 16 bits each, oldest first
+
+  __device__ __forceinline__ TileFetch(const AttnArgs& a_, const Parts& p_, bool any)
+      : a(a_), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), p(p_), more(any), masks(0) { if (any) enter(); }
+
+  // Begins at the current part's first tile for this warp, or that of a later part.
+  __device__ __forceinline__ void enter() {
+    while (p.tile0 + warp >= p.tile1) {
+      more = p.next(a);
+      if (!more) return;
+    }
+    next = p.tile0 + warp;
+    have = 0;
+    kb = (const T*)a.k_cache + p.kvh * a.kc_sh;
+    vb = (const T*)a.v_cache + p.kvh * a.vc_sh;
+  }
+
+  __device__ __forceinline__ void lookup(int tok, bool on) {
+    pg = -1;
+    sl = 0;
+    if (on) {
+      const int w = tok / a.page_size;
+      sl = tok - w * a.page_size;
+      pg = a.table[(int64_t)p.b * a.t_sb + w];
+      if (pg < 0 || pg >= a.n_pages) {
+        set_status(a.status, kBadArgument, kSiteAttnPage);
+        pg = -1;
+      }
+    }
+  }
+
+  // Starts the warp's copies of the next tile into the ring at `stage`.
+  __device__ __forceinline__ void fetch(uint32_t stage) {
+    uint32_t mask = 0;
+    if (more) {
+      int page = 0, slot = 0;
+      if constexpr (PAGE16) {
+        if (have == 0) {
+          const int tile = next + lane * kAttnWarps;
+          lookup(tile * kTile, tile < p.tile1);
+          have = 32;
+        }
+        page = __shfl_sync(0xffffffffu, pg, 32 - have);
+        slot = __shfl_sync(0xffffffffu, sl, 32 - have);
+        --have;
+        mask = page < 0 ? 0u : (1u << min(kTile, p.len - next * kTile)) - 1u;
+      } else {
+        const int tok = next * kTile + lane;
+        lookup(tok, lane < kTile && tok < p.len);
+        mask = __ballot_sync(0xffffffffu, pg >= 0) & 0xFFFFu;
+      }
+      if (PAGE16 && mask == 0xFFFFu) {
+        const T* kp = kb + (int64_t)page * a.kc_sp + (int64_t)slot * a.kc_ss;
+        const T* vp = vb + (int64_t)page * a.vc_sp + (int64_t)slot * a.vc_ss;
+        if constexpr (D != 96) {  // whole rows a copy: pointers advance by the same step
+          constexpr int kRows = 32 / L::kPieces;
+          const int t0 = lane / L::kPieces, piece = lane % L::kPieces;
+          kp += t0 * a.kc_ss + piece * 8;
+          vp += t0 * a.vc_ss + piece * 8;
+#pragma unroll
+          for (int i = 0; i < L::kCopies; ++i) {
+            cp16(stage + L::k_at(i * kRows + t0, piece), kp);
+            kp += kRows * a.kc_ss;
+          }
+#pragma unroll
+          for (int i = 0; i < L::kCopies; ++i) {
+            cp16(stage + L::v_at(i * kRows + t0, piece), vp);
+            vp += kRows * a.vc_ss;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < L::kCopies; ++i) {
+            const int u = i * 32 + lane, t = u / L::kPieces, piece = u - t * L::kPieces;
+            cp16(stage + L::k_at(t, piece), kp + t * a.kc_ss + piece * 8);
+            cp16(stage + L::v_at(t, piece), vp + t * a.vc_ss + piece * 8);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < L::kCopies; ++i) {
+          const int u = i * 32 + lane, t = u / L::kPieces, piece = u - t * L::kPieces;
+          const int tp = PAGE16 ? page : __shfl_sync(0xffffffffu, pg, t);
+          const int64_t ts = PAGE16 ? slot + t : __shfl_sync(0xffffffffu, sl, t);
+          const bool on = mask >> t & 1;
+          cp16_if(stage + L::k_at(t, piece), on ? kb + tp * a.kc_sp + ts * a.kc_ss + piece * 8 : kb, on);
+          cp16_if(stage + L::v_at(t, piece), on ? vb + tp * a.vc_sp + ts * a.vc_ss + piece * 8 : vb, on);
+        }
+      }
+      next += kAttnWarps;
+      if (next >= p.tile1) {
+        more = p.next(a);
+        if (more) enter();
+      }
+    }
+    cp_commit();
+    masks = masks >> 16 | (uint64_t)mask << (16 * (S - 1));
+  }
+};
+
+template <typename T, int D, int NG, bool PAGE16>
+__global__ void __launch_bounds__(32 * kAttnWarps, NG == 1 ? 3 : 2) attn_mma_kernel(const AttnArgs a) {
+  using W = TileFetch<T, D, PAGE16>;
+  using L = Tile<D>;
+  constexpr int KC = D / 32, MT = D / 16;
+  constexpr int kPitchO = D + 4;  // floats of a row of s_o
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ float s_m[kAttnWarps][8 * NG], s_l[kAttnWarps][8 * NG];
+  // rows begin at multiples of their pitch, so that a piece's index can be xor-ed into its address
+  unsigned char* smem = smem_raw + (-(uint32_t)__cvta_generic_to_shared(smem_raw) & 255u);
+  static_assert(W::S <= 4, "masks");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
+  const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(smem) + warp * W::S * L::kStage;
+  const uint32_t ring1 = ring0 + W::S * L::kStage;
+  float* s_o = reinterpret_cast<float*>(smem + kAttnWarps * W::S * L::kStage);  // [warp][4 heads][kPitchO]
+  // this lane's places in a tile: key pieces of tokens r and r + 8, and its row address for ldmatrix
+  const int k_lane = L::k_at(r, j);
+  const int v_lane = L::v_at((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
+  uint32_t stage = ring0;
+  Parts p;
+  bool more = p.first(a);
+  W w(a, p, more);
+#pragma unroll 1
+  for (int i = 0; i < W::S; ++i) w.fetch(ring0 + i * L::kStage);
+  for (; more; more = p.next(a)) {
+    uint4 q[NG][KC];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int row = g * 8 + r;
+        q[g][c] = make_uint4(0, 0, 0, 0);
+        if (row < p.rows) {
+          const T* qp = (const T*)a.q + p.b * a.q_sb + (p.row0 + row) * a.q_sh + 32 * c + 8 * j;
+          q[g][c] = *reinterpret_cast<const uint4*>(qp);
+        }
+      }
+    float o[NG][MT][4];            // values 16 t + r (+ 8) of heads 2j, 2j + 1
+    float m[NG][2], l[NG][2];      // of heads 2j, 2j + 1; the sum over this lane's tokens only
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      m[g][0] = m[g][1] = -INFINITY;
+      l[g][0] = l[g][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) o[g][t][0] = o[g][t][1] = o[g][t][2] = o[g][t][3] = 0.f;
+    }
+#pragma unroll 1
+    for (int tile = p.tile0 + warp; tile < p.tile1; tile += kAttnWarps) {
+      cp_wait<W::S - 1>();
+      __syncwarp();
+      const uint32_t mask = (uint32_t)w.masks & 0xFFFFu;
+      float s[NG][2][4];           // two sums, so that products need not wait for one another
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[g][0][i] = s[g][1][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint4 x = lds16((stage + k_lane) ^ (c << 6)), y = lds16(((stage + k_lane) ^ (c << 6)) + 8 * L::kPitch);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          Mma<T>::run(s[g][0], x.x, y.x, x.y, y.y, q[g][c].x, q[g][c].y);
+          Mma<T>::run(s[g][1], x.z, y.z, x.w, y.w, q[g][c].z, q[g][c].w);
+        }
+      }
+      uint32_t hi[NG][2], lo[NG][2];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float z[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = (s[g][0][i] + s[g][1][i]) * a.scale_log2;
+        if (mask != 0xFFFFu) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[i] = mask >> (r + 8 * (i >> 1)) & 1 ? z[i] : -INFINITY;
+        }
+        float mx[2] = {fmaxf(z[0], z[2]), fmaxf(z[1], z[3])};
+        if (__any_sync(0xffffffffu, mx[0] > m[g][0] + 8.f || mx[1] > m[g][1] + 8.f)) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], x));
+            const float mn = fmaxf(m[g][n], mx[n]), alpha = ex2(m[g][n] - max_or_zero(mn));
+            m[g][n] = mn;
+            l[g][n] *= alpha;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+              o[g][t][n] *= alpha;
+              o[g][t][n + 2] *= alpha;
+            }
+          }
+        }
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = ex2(z[i] - max_or_zero(m[g][i & 1]));
+        l[g][0] += e[0] + e[2];
+        l[g][1] += e[1] + e[3];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = Mma<T>::pack(e[2 * h] * Mma<T>::kLow, e[2 * h + 1] * Mma<T>::kLow);
+          const float2 f = Mma<T>::unpack(x);
+          hi[g][h] = transpose8x8(x);
+          lo[g][h] = transpose8x8(Mma<T>::pack(e[2 * h] - f.x, e[2 * h + 1] - f.y));
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const uint4 x = ldmatrix4t((stage + v_lane) ^ (t << 5));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          Mma<T>::run(o[g][t], x.x, x.y, x.z, x.w, hi[g][0], hi[g][1]);
+          Mma<T>::run(o[g][t], x.x, x.y, x.z, x.w, lo[g][0], lo[g][1]);
+        }
+      }
+      __syncwarp();  // every lane has read the tile
+      w.fetch(stage);
+      stage = stage + L::kStage == ring1 ? ring0 : stage + L::kStage;
+    }
+    // the warps' results, joined in order, 4 heads at a time
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[g][n] += __shfl_xor_sync(0xffffffffu, l[g][n], x);
+        if (r == 0) {
+          s_m[warp][g * 8 + 2 * j + n] = m[g][n];
+          s_l[warp][g * 8 + 2 * j + n] = l[g][n];
+        }
+      }
+#pragma unroll
+    for (int h4 = 0; h4 < 2 * NG; ++h4) {
+      if (4 * h4 >= p.rows) break;
+      if ((j >> 1) == (h4 & 1)) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float* so = s_o + (warp * 4 + 2 * (j & 1) + n) * kPitchO + r;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            so[16 * t] = o[h4 / 2][t][n];
+            so[16 * t + 8] = o[h4 / 2][t][n + 2];
+          }
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < min(4, p.rows - 4 * h4) * (D / 4); i += blockDim.x) {
+        const int gl = i / (D / 4), d = i % (D / 4) * 4, g = 4 * h4 + gl;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int y = 0; y < kAttnWarps; ++y) mx = fmaxf(mx, s_m[y][g]);
+        float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < kAttnWarps; ++y) {
+          const float e = ex2(s_m[y][g] - max_or_zero(mx));
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (y * 4 + gl) * kPitchO + d);
+          sum += s_l[y][g] * e;
+          acc[0] += x.x * e; acc[1] += x.y * e; acc[2] += x.z * e; acc[3] += x.w * e;
+        }
+        if (p.slot < 0) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          T* op = (T*)a.out + p.b * a.o_sb + (p.row0 + g) * a.o_sh + d;
+          const uint2 y = make_uint2(Mma<T>::pack(acc[0] * inv, acc[1] * inv), Mma<T>::pack(acc[2] * inv, acc[3] * inv));
+          *reinterpret_cast<uint2*>(op) = y;
+        } else {
+          const int64_t rr = (int64_t)p.slot * a.rows + g;
+          *reinterpret_cast<float4*>(a.ws_o + rr * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (d == 0) {
+            a.ws_ml[2 * rr] = mx;
+            a.ws_ml[2 * rr + 1] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  zero_empty<T>(a);
+}
+
+// Combines the parts of each (sequence, query head) that several CTAs share, in list order. One
+// block per sequence and query head: the weights of up to 128 parts are made at once, then threads
+// add the parts' rows, VEC values each, in as many interleaved sums as the block has room for.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+  __shared__ float s_w[128];
+  __shared__ float s_red[2][4];
+  __shared__ alignas(16) float s_acc[128 * VEC];
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq;
   const int tiles = seq_tiles(a, b);
-  T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
-  if (tiles == 0) {
-    for (int d = threadIdx.x; d < a.D; d += blockDim.x) out[d] = from_f32<T>(0.f);
-    return;
-  }
   const int kvh = h / a.G, sub = (h - kvh * a.G) / a.rows, g = h - kvh * a.G - sub * a.rows;
-  const int64_t before = tiles_before(a, b);
-  const int64_t per = tiles_per_cta(a, before + tiles_before(a, a.B) - before);
+  int64_t before, all;
+  tiles_before_and_all(a, b, before, all);
+  const int64_t per = tiles_per_cta(a, all);
   const int64_t s0 = before * a.units + (int64_t)(kvh * a.subs + sub) * tiles, s1 = s0 + tiles;
-  const int64_t c0 = s0 / per, c1 = (s1 - 1) / per;
-  if (c0 == c1) return;  // finished by the one CTA that had it
-  for (int d = threadIdx.x; d < a.D; d += blockDim.x) {
-    float m = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int64_t c = c0; c <= c1; ++c) {
-      // the first CTA has the rows in its last slot unless its run starts there
-      const int64_t r = (2 * c + (c * per < s0 ? 1 : 0)) * a.rows + g;
-      const float pm = a.ws_ml[2 * r], pl = a.ws_ml[2 * r + 1], po = a.ws_o[r * a.D + d];
-      const float mx = fmaxf(m, pm), base = max_or_zero(mx);
-      const float e0 = exp2f(m - base), e1 = exp2f(pm - base);
-      sum = sum * e0 + pl * e1;
-      acc = acc * e0 + po * e1;
-      m = mx;
+  const int c0 = (int)(s0 / per), c1 = (int)((s1 - 1) / per);
+  // launched while the main kernel still runs; its parts are complete behind this point
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tiles == 0 || c0 == c1) return;  // empty, or finished by the one CTA that had it
+  // the first CTA has the rows in its last slot unless its run starts there
+  const int first = 2 * c0 + (c0 * per < s0 ? 1 : 0);
+  auto row_of = [&](int i) { return (int64_t)(i == 0 ? first : 2 * (c0 + i)) * a.rows + g; };
+  const int n = c1 - c0 + 1;
+  const int lanes = (a.D + VEC - 1) / VEC, warp = threadIdx.x >> 5;
+  const int nway = lanes >= 128 ? 1 : 128 / lanes;
+  const int way = threadIdx.x / lanes, d = (threadIdx.x - way * lanes) * VEC;
+  const bool on = way < nway;
+  float m = -INFINITY, sum = 0.f, acc[2][VEC];  // a block of 128 threads holds up to 256 values in two rounds
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 128) {
+    const int k = min(128, n - i0);
+    const int64_t r = row_of(i0 + min((int)threadIdx.x, k - 1));
+    const float pm = (int)threadIdx.x < k ? a.ws_ml[2 * r] : -INFINITY;
+    const float pl = (int)threadIdx.x < k ? a.ws_ml[2 * r + 1] : 0.f;
+    const float wm = warp_max(pm);
+    if ((threadIdx.x & 31) == 0) s_red[0][warp] = wm;
+    __syncthreads();
+    const float mn = fmaxf(m, fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3])));
+    const float alpha = exp2f(m - max_or_zero(mn));
+    const float w = exp2f(pm - max_or_zero(mn));
+    m = mn;
+    s_w[threadIdx.x] = w;
+    const float ws = warp_sum(pl * w);
+    if ((threadIdx.x & 31) == 0) s_red[1][warp] = ws;
+    __syncthreads();
+    sum = sum * alpha + ((s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]));
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      acc[0][e] *= alpha;
+      acc[1][e] *= alpha;
     }
-    out[d] = from_f32<T>(sum == 0.f ? 0.f : acc / sum);
+    if (on) {
+#pragma unroll 8
+      for (int i = way; i < k; i += nway) {
+        const float f = s_w[i];
+        const float* src = a.ws_o + row_of(i0 + i) * a.D + d;
+        if constexpr (VEC == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          acc[0][0] += x.x * f; acc[0][1] += x.y * f; acc[0][2] += x.z * f; acc[0][3] += x.w * f;
+        } else {
+          acc[0][0] += src[0] * f;
+          if (d + 128 < a.D) acc[1][0] += src[128] * f;
+        }
+      }
+    }
+    __syncthreads();
   }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) s_acc[threadIdx.x * VEC + e] = acc[0][e];
+  __syncthreads();
+  if (way != 0 || d >= a.D) return;
+  T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    float x = acc[0][e];
+    for (int y = 1; y < nway; ++y) x += s_acc[(y * lanes) * VEC + d + e];
+    out[d + e] = from_f32<T>(x * inv);
+  }
+  if (VEC == 1 && d + 128 < a.D) out[d + 128] = from_f32<T>(acc[1][0] * inv);
 }
 
 }  // namespace nfb
@@ -455,6 +954,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
 using namespace nfb;
 
 namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T, int V>
 int launch_append(AppendArgs& a, cudaStream_t st) {
@@ -476,33 +977,95 @@ int launch_plain(const AttnArgs& a, cudaStream_t st) {
   return (int)cudaGetLastError();
 }
 
-template <typename T>
-int launch_attn(const AttnArgs& a, cudaStream_t st) {
-  int rc;
-  if (a.D <= 64) rc = launch_plain<T, 2>(a, st);
-  else if (a.D <= 128) rc = launch_plain<T, 4>(a, st);
-  else rc = launch_plain<T, 8>(a, st);
-  if (rc != 0) return rc;
-  attn_join_kernel<T><<<(unsigned)(a.B * a.Hq), 128, 0, st>>>(a);
+template <typename T, int D, int NG, bool PAGE16>
+int launch_mma_one(const AttnArgs& a, cudaStream_t st) {
+  constexpr int kSmem = attn_smem<D>();
+  static uint64_t ready = 0;  // one bit per device (an attribute set twice does no harm)
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(attn_mma_kernel<T, D, NG, PAGE16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess && dev < 64) ready |= 1ull << dev;
+  }
+  if (e != cudaSuccess) return (int)e;
+  attn_mma_kernel<T, D, NG, PAGE16><<<a.ctas, 32 * kAttnWarps, kSmem, st>>>(a);
   return (int)cudaGetLastError();
 }
 
-// The split of a call into units and CTAs; the same for the workspace query and the launch.
-void plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, int sms, AttnArgs& a) {
+template <typename T, int D>
+int launch_mma(const AttnArgs& a, cudaStream_t st) {
+  const bool p16 = a.page_size % kTile == 0;
+  if (a.rows <= 8) return p16 ? launch_mma_one<T, D, 1, true>(a, st) : launch_mma_one<T, D, 1, false>(a, st);
+  return p16 ? launch_mma_one<T, D, 2, true>(a, st) : launch_mma_one<T, D, 2, false>(a, st);
+}
+
+template <typename T>
+int launch_attn(const AttnArgs& a, bool mma, cudaStream_t st) {
+  int rc;
+  if constexpr (sizeof(T) == 2) {
+    if (mma) {
+      switch (a.D) {
+        case 32: rc = launch_mma<T, 32>(a, st); break;
+        case 64: rc = launch_mma<T, 64>(a, st); break;
+        case 96: rc = launch_mma<T, 96>(a, st); break;
+        default: rc = launch_mma<T, 128>(a, st); break;
+      }
+    }
+  }
+  if (!mma) {
+    if (a.D <= 64) rc = launch_plain<T, 2>(a, st);
+    else if (a.D <= 128) rc = launch_plain<T, 4>(a, st);
+    else rc = launch_plain<T, 8>(a, st);
+  }
+  if (rc != 0 || a.whole || a.ctas == 1) return rc;  // nothing to join
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hq));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const bool vec = a.D % 4 == 0 && aligned16(a.ws_o);
+  return (int)(vec ? cudaLaunchKernelEx(&cfg, attn_join_kernel<T, 4>, a) : cudaLaunchKernelEx(&cfg, attn_join_kernel<T, 1>, a));
+}
+
+// The split of a call into units and CTAs. Short caches (up to 48 tiles a sequence): one CTA for each
+// (sequence, unit), one launch (400 tokens, 8 sequences of 8 key heads of 128: 7.6 us, divided 10 us;
+// 1000 tokens, 4 sequences: 13.1 us, divided 11.5 us). Else the list is divided over as many CTAs as
+// the GPU holds; where there is much work for each of them and many sequences, over twice as many,
+// which evens out SMs of different speed (64 ragged sequences of up to 3392: 78 us against 84; but one
+// of 131001: 90 us against 97, its join grows).
+void plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool mma, int sms, AttnArgs& a) {
   a.B = (int)B;
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
   a.D = (int)D;
   a.G = (int)(Hq / Hkv);
-  a.rows = a.G == 1 ? 1 : 4;
-  a.subs = (a.G + a.rows - 1) / a.rows;
+  if (mma) {
+    a.subs = (a.G + 15) / 16;
+    a.rows = (a.G + a.subs - 1) / a.subs;
+  } else {
+    a.rows = a.G == 1 ? 1 : 4;
+    a.subs = (a.G + a.rows - 1) / a.rows;
+  }
   a.units = a.Hkv * a.subs;
+  if (capacity > INT_MAX - 2 * kTile) capacity = INT_MAX - 2 * kTile;
+  const int64_t pairs = B * a.units, per_seq = (capacity + kTile - 1) / kTile;
+  const int64_t slots = (int64_t)sms * (!mma ? 4 : a.rows <= 8 ? 3 : 2);
   a.min_tiles = kAttnWarps;
-  const int64_t most = B * a.units * ((capacity + kTile - 1) / kTile);
-  const int64_t want = (most + a.min_tiles - 1) / a.min_tiles;
-  const int64_t slots = (int64_t)sms * 4;
-  a.ctas = (int)(want < 1 ? 1 : want < slots ? want : slots);
+  a.whole = per_seq <= 48 && pairs <= INT_MAX;
+  if (a.whole) {
+    a.ctas = (int)pairs;
+  } else {
+    const int64_t want = (pairs * per_seq + a.min_tiles - 1) / a.min_tiles;
+    const int64_t most = pairs * per_seq >= 96 * slots && 4 * pairs >= slots ? 2 * slots : slots;
+    a.ctas = (int)(want < 1 ? 1 : want < most ? want : most);
+  }
 }
+
+int64_t ws_floats(const AttnArgs& a) { return a.whole ? 0 : (int64_t)2 * a.ctas * a.rows * (a.D + 2); }
 
 }  // namespace
 
@@ -542,8 +1105,10 @@ NFB_API int nfb_append_kv(int dtype, const void* q, const void* k, const void* v
 
 NFB_API int64_t nfb_paged_attn_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity) {
   AttnArgs a;
-  plan(B, Hq, Hkv, D, capacity, nfb_num_sms(), a);
-  return (int64_t)2 * a.ctas * a.rows * (D + 2);
+  plan(B, Hq, Hkv, D, capacity, false, nfb_num_sms(), a);
+  const int64_t n = ws_floats(a);
+  plan(B, Hq, Hkv, D, capacity, true, nfb_num_sms(), a);
+  return n > ws_floats(a) ? n : ws_floats(a);
 }
 
 // dims: B, Hq, Hkv, D, page_size, n_pages, table_width, then the strides q (b, h), out (b, h),
@@ -557,7 +1122,13 @@ NFB_API int nfb_paged_attn(int dtype, const void* q, const void* k_cache, const 
   const int64_t B = dims[0], Hq = dims[1], Hkv = dims[2], D = dims[3];
   if (B == 0 || Hq == 0) return 0;
   if (Hkv < 1 || Hq % Hkv || D < 1 || D > 256 || dims[4] < 1 || B * Hq > INT_MAX) return (int)cudaErrorInvalidValue;
-  plan(B, Hq, Hkv, D, dims[4] * dims[6], nfb_num_sms(), a);
+  // the tensor-core kernel reads 16-byte pieces of rows of 16-bit values
+  bool mma = dtype != kF32 && (D == 32 || D == 64 || D == 96 || D == 128) && aligned16(q) && aligned16(k_cache) &&
+             aligned16(v_cache) && aligned16(ws) && dims[9] % 4 == 0 && dims[10] % 4 == 0 &&
+             (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+  const int piece[] = {7, 8, 11, 12, 13, 14, 15, 16};
+  for (int i : piece) mma = mma && dims[i] % 8 == 0;
+  plan(B, Hq, Hkv, D, dims[4] * dims[6], mma, nfb_num_sms(), a);
   a.page_size = (int)dims[4]; a.n_pages = (int)dims[5]; a.table_width = (int)dims[6];
   a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.out = out; a.table = table; a.lengths = lengths;
   a.ws_o = ws;
@@ -570,9 +1141,9 @@ NFB_API int nfb_paged_attn(int dtype, const void* q, const void* k_cache, const 
   a.t_sb = dims[17];
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case kF32: return launch_attn<float>(a, st);
-    case kBF16: return launch_attn<__nv_bfloat16>(a, st);
-    case kF16: return launch_attn<__half>(a, st);
+    case kF32: return launch_attn<float>(a, mma, st);
+    case kBF16: return launch_attn<__nv_bfloat16>(a, mma, st);
+    case kF16: return launch_attn<__half>(a, mma, st);
   }
   return (int)cudaErrorInvalidValue;
 }
