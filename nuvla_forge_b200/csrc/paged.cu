@@ -26,9 +26,16 @@ enum PagedSite : uint32_t { kSiteAppendPos = 1, kSiteAppendPage = 2, kSiteAppend
 // tables, so far positions lose nothing to a product p * frequency in fp32; the turn is computed
 // in fp32 and rounded once to the storage type.
 //
-// One unit of work is V pairs (two vectors) of a rotated head or one vector of what is copied as it
-// is; a block of 256 threads takes the units of one token, or of several where a token has few.
+// The call is bound by its bytes (each input read, each output written once), so it is shaped like a
+// copy: one unit of work a thread, no loop, no shared memory, few registers, the data on its way
+// before the token's place is looked up. A unit is two vectors (of 16 bytes where everything is
+// aligned) of one head: V pairs of a rotated head, or what is copied as it is. Threads that keep the
+// angles for several heads or tokens were slower (8 contexts of 3392 tokens, 16 + 8 heads of 128:
+// 79 to 114 us against 78 us, 5.7 TB/s), for want of loads in flight; at 40 registers 12 blocks of 128
+// threads are resident.
 // ---------------------------------------------------------------------------------------------
+constexpr int kAppendThreads = 128;
+
 struct AppendArgs {
   const void *q, *k, *v;
   void *q_out, *k_cache, *v_cache;
@@ -37,7 +44,7 @@ struct AppendArgs {
   uint32_t* status;
   int64_t tokens;  // B * T
   int T, Hq, Hkv, D, half, interleaved, page_size, n_pages, table_width, rope_rows;
-  int units, units_rot, tokens_per_block;
+  int units, units_rot, units_v;  // of a token; of a head of q or k; of a head of v
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
   int64_t kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, t_sb;
 };
@@ -65,101 +72,106 @@ __device__ __forceinline__ void chunk_store(T* p, const Chunk<T, V>& c) {
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
-  const int local = threadIdx.x / a.units;
-  const int64_t token = (int64_t)blockIdx.x * a.tokens_per_block + local;
-  if (local >= a.tokens_per_block || token >= a.tokens) return;
-  const int b = (int)(token / a.T), t = (int)(token - (int64_t)b * a.T);
+__device__ __forceinline__ Chunk<T, V> chunk_load_once(const T* p) {
+  if constexpr (V * sizeof(T) == 16) {
+    uint4 u;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+    return *reinterpret_cast<Chunk<T, V>*>(&u);
+  } else {
+    return chunk_load<T, V>(p);
+  }
+}
+
+// Turns V pairs: (x1[i], x2[i]), or the neighbours among the 2 V values of x1, x2.
+template <typename T, int V, bool PAIRS>
+__device__ __forceinline__ void turn(Chunk<T, V>& c1, Chunk<T, V>& c2, const float* c, const float* s) {
+  float x[2 * V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    x[i] = to_f32(c1.v[i]);
+    x[V + i] = to_f32(c2.v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int ia = PAIRS ? 2 * i : i, ib = PAIRS ? 2 * i + 1 : V + i;
+    const T ra = from_f32<T>(x[ia] * c[i] - x[ib] * s[i]), rb = from_f32<T>(x[ib] * c[i] + x[ia] * s[i]);
+    (ia < V ? c1.v[ia % V] : c2.v[ia % V]) = ra;
+    (ib < V ? c1.v[ib % V] : c2.v[ib % V]) = rb;
+  }
+}
+
+template <typename T, int V, bool PAIRS>
+__global__ void __launch_bounds__(kAppendThreads, 12) append_kernel(const AppendArgs a) {
+  const int64_t idx = (int64_t)blockIdx.x * kAppendThreads + threadIdx.x;
+  const int64_t token = idx <= INT_MAX ? (int)((uint32_t)idx / (uint32_t)a.units) : idx / a.units;
+  if (token >= a.tokens) return;
+  int u = (int)(idx - token * a.units);
+  const int b = token <= INT_MAX ? (int)((uint32_t)token / (uint32_t)a.T) : (int)(token / a.T);
+  const int t = (int)(token - (int64_t)b * a.T);
   const bool live = a.counts == nullptr || t < a.counts[b];
+  const int q_units = a.Hq * a.units_rot, k_units = a.Hkv * a.units_rot;
+  const int kind = u < q_units ? 0 : u < q_units + k_units ? 1 : 2;
+  if (kind != 0 && !live) return;
+  u -= kind == 0 ? 0 : kind == 1 ? q_units : q_units + k_units;
+  const int per = kind == 2 ? a.units_v : a.units_rot;
+  const int h = u / per, e = u - h * per;
+  // the unit's vectors: a rotated pair of vectors, or up to two neighbours of the rest
+  const int n_pair = kind == 2 ? 0 : a.half / V;
+  const bool turned = e < n_pair;
+  const int rest = (kind == 2 ? 0 : 2 * a.half) + (e - n_pair) * 2 * V;
+  const int o1 = turned ? (PAIRS ? 2 * e * V : e * V) : rest;
+  const int o2 = turned ? (PAIRS ? o1 + V : a.half + e * V) : rest + V;
+  const bool two = turned || o2 < a.D;
+  const T* src = kind == 0   ? (const T*)a.q + b * a.q_sb + t * a.q_st + h * a.q_sh
+                 : kind == 1 ? (const T*)a.k + b * a.k_sb + t * a.k_st + h * a.k_sh
+                             : (const T*)a.v + b * a.v_sb + t * a.v_st + h * a.v_sh;
+  Chunk<T, V> c1 = chunk_load_once<T, V>(src + o1), c2;
+  if (two) c2 = chunk_load_once<T, V>(src + o2);
   const int64_t pos = (int64_t)a.starts[b] + t;
-  // where the token goes; page < 0: nowhere
-  int page = -1, slot = 0;
-  if (live) {
+  int64_t row = pos;
+  bool stored = live;
+  if (a.half > 0 && (pos < 0 || pos >= a.rope_rows)) {
+    // padding behind the count takes the tables' nearest row; a live token must have its own
+    if (live) set_status(a.status, kBadArgument, kSiteAppendRope);
+    stored = false;
+    row = pos < 0 ? 0 : a.rope_rows - 1;
+  }
+  T* dst;
+  if (kind == 0) {
+    dst = (T*)a.q_out + (token * a.Hq + h) * a.D;
+  } else {
+    if (!stored) return;
     if (pos < 0 || pos >= (int64_t)a.table_width * a.page_size) {
       set_status(a.status, kBadArgument, kSiteAppendPos);
-    } else {
-      page = a.table[(int64_t)b * a.t_sb + pos / a.page_size];
-      slot = (int)(pos % a.page_size);
-      if (page < 0 || page >= a.n_pages) {
-        set_status(a.status, kBadArgument, kSiteAppendPage);
-        page = -1;
-      }
+      return;
     }
+    const int w = pos <= INT_MAX ? (int)((uint32_t)pos / (uint32_t)a.page_size) : (int)(pos / a.page_size);
+    const int slot = (int)(pos - (int64_t)w * a.page_size);
+    const int page = a.table[(int64_t)b * a.t_sb + w];
+    if (page < 0 || page >= a.n_pages) {
+      set_status(a.status, kBadArgument, kSiteAppendPage);
+      return;
+    }
+    dst = kind == 1 ? (T*)a.k_cache + page * a.kc_sp + slot * a.kc_ss + h * a.kc_sh
+                    : (T*)a.v_cache + page * a.vc_sp + slot * a.vc_ss + h * a.vc_sh;
   }
-  int64_t row = pos;
-  if (a.half > 0 && (row < 0 || row >= a.rope_rows)) {
-    // padding behind the count takes the table's last row; a live token must have a row of its own
-    if (live) {
-      set_status(a.status, kBadArgument, kSiteAppendRope);
-      page = -1;
-    }
-    row = row < 0 ? 0 : a.rope_rows - 1;
-  }
-  const int n_pair = a.half / V;
-  const int rot_units = (a.Hq + a.Hkv) * a.units_rot;
-  for (int u = a.tokens_per_block > 1 ? threadIdx.x - local * a.units : threadIdx.x; u < a.units;
-       u += a.tokens_per_block > 1 ? a.units : blockDim.x) {
-    const T* src;
-    T* dst;
-    int e;  // index of the unit within its head
-    bool rot = false;
-    if (u < rot_units) {
-      int h = u / a.units_rot;
-      e = u - h * a.units_rot;
-      rot = e < n_pair;
-      if (h < a.Hq) {
-        src = (const T*)a.q + b * a.q_sb + t * a.q_st + h * a.q_sh;
-        dst = (T*)a.q_out + (token * a.Hq + h) * a.D;
-      } else {
-        if (page < 0) continue;
-        h -= a.Hq;
-        src = (const T*)a.k + b * a.k_sb + t * a.k_st + h * a.k_sh;
-        dst = (T*)a.k_cache + page * a.kc_sp + slot * a.kc_ss + h * a.kc_sh;
-      }
-    } else {
-      if (page < 0) continue;
-      const int w = u - rot_units, per = a.D / V;
-      const int h = w / per;
-      e = w - h * per;
-      src = (const T*)a.v + b * a.v_sb + t * a.v_st + h * a.v_sh;
-      dst = (T*)a.v_cache + page * a.vc_sp + slot * a.vc_ss + h * a.vc_sh;
-      chunk_store<T, V>(dst + e * V, chunk_load<T, V>(src + e * V));
-      continue;
-    }
-    if (!rot) {
-      const int off = 2 * a.half + (e - n_pair) * V;
-      chunk_store<T, V>(dst + off, chunk_load<T, V>(src + off));
-      continue;
-    }
-    const int o1 = a.interleaved ? 2 * e * V : e * V;
-    const int o2 = a.interleaved ? o1 + V : a.half + e * V;
-    Chunk<T, V> c1 = chunk_load<T, V>(src + o1), c2 = chunk_load<T, V>(src + o2);
-    const float* cs = a.cos + row * a.half + e * V;
-    const float* sn = a.sin + row * a.half + e * V;
-    float x[2 * V];
+  if (turned) {
+    const float *cos = a.cos + row * a.half + e * V, *sin = a.sin + row * a.half + e * V;
+    float cs[V], sn[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      x[i] = to_f32(c1.v[i]);
-      x[V + i] = to_f32(c2.v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int ia = a.interleaved ? 2 * i : i, ib = a.interleaved ? 2 * i + 1 : V + i;
-      const float c = cs[i], s = sn[i];
-      // selected by constant indices in both layouts, so x stays in registers
-      const float xa = a.interleaved ? x[2 * i] : x[i], xb = a.interleaved ? x[2 * i + 1] : x[V + i];
-      const T ra = from_f32<T>(xa * c - xb * s), rb = from_f32<T>(xb * c + xa * s);
-      if (a.interleaved) {
-        if (ia < V) c1.v[ia < V ? ia : 0] = ra; else c2.v[ia >= V ? ia - V : 0] = ra;
-        if (ib < V) c1.v[ib < V ? ib : 0] = rb; else c2.v[ib >= V ? ib - V : 0] = rb;
+    for (int k = 0; k < V; k += (V % 4 == 0 ? 4 : 1)) {
+      if constexpr (V % 4 == 0) {
+        *reinterpret_cast<float4*>(cs + k) = __ldg(reinterpret_cast<const float4*>(cos + k));
+        *reinterpret_cast<float4*>(sn + k) = __ldg(reinterpret_cast<const float4*>(sin + k));
       } else {
-        c1.v[i] = ra;
-        c2.v[i] = rb;
+        cs[k] = __ldg(cos + k);
+        sn[k] = __ldg(sin + k);
       }
     }
-    chunk_store<T, V>(dst + o1, c1);
-    chunk_store<T, V>(dst + o2, c2);
+    turn<T, V, PAIRS>(c1, c2, cs, sn);
   }
+  chunk_store<T, V>(dst + o1, c1);
+  if (two) chunk_store<T, V>(dst + o2, c2);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -959,14 +971,16 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 template <typename T, int V>
 int launch_append(AppendArgs& a, cudaStream_t st) {
-  a.units_rot = a.half / V + (a.D - 2 * a.half) / V;
-  const int64_t units = (int64_t)(a.Hq + a.Hkv) * a.units_rot + (int64_t)a.Hkv * (a.D / V);
-  if (units > INT_MAX / 2) return (int)cudaErrorInvalidValue;
+  const int rest = (a.D - 2 * a.half) / V;
+  a.units_rot = a.half / V + (rest + 1) / 2;
+  a.units_v = (a.D / V + 1) / 2;
+  const int64_t units = (int64_t)(a.Hq + a.Hkv) * a.units_rot + (int64_t)a.Hkv * a.units_v;
+  if (units > INT_MAX) return (int)cudaErrorInvalidValue;
   a.units = (int)units;
-  a.tokens_per_block = units >= 256 ? 1 : 256 / (int)units;
-  const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
-  if (blocks > INT_MAX) return (int)cudaErrorInvalidValue;
-  append_kernel<T, V><<<(unsigned)blocks, 256, 0, st>>>(a);
+  if (a.tokens > ((int64_t)INT_MAX * kAppendThreads) / units) return (int)cudaErrorInvalidValue;
+  const int64_t blocks = (a.tokens * units + kAppendThreads - 1) / kAppendThreads;
+  if (a.interleaved) append_kernel<T, V, true><<<(unsigned)blocks, kAppendThreads, 0, st>>>(a);
+  else append_kernel<T, V, false><<<(unsigned)blocks, kAppendThreads, 0, st>>>(a);
   return (int)cudaGetLastError();
 }
 
@@ -1094,11 +1108,16 @@ NFB_API int nfb_append_kv(int dtype, const void* q, const void* k, const void* v
   if (a.tokens == 0 || a.D == 0 || a.Hkv == 0) return 0;
   if (2 * a.half > a.D || a.page_size < 1 || (a.half > 0 && (a.rope_rows < 1 || !cos || !sin)))
     return (int)cudaErrorInvalidValue;
+  // 16-byte vectors where every row, and every half of a rotated one, begins on 16 bytes
+  const int V = dtype == kF32 ? 4 : 8;
+  bool vec = a.D % V == 0 && a.half % V == 0 && aligned16(k) && aligned16(v) && aligned16(k_cache) && aligned16(v_cache) &&
+             (!q || (aligned16(q) && aligned16(q_out))) && (a.half == 0 || (aligned16(cos) && aligned16(sin)));
+  for (int i = q ? 11 : 14; i < 26; ++i) vec = vec && dims[i] % V == 0;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case kF32: return launch_append<float, 1>(a, st);
-    case kBF16: return launch_append<__nv_bfloat16, 1>(a, st);
-    case kF16: return launch_append<__half, 1>(a, st);
+    case kF32: return vec ? launch_append<float, 16 / sizeof(float)>(a, st) : launch_append<float, 1>(a, st);
+    case kBF16: return vec ? launch_append<__nv_bfloat16, 16 / sizeof(__nv_bfloat16)>(a, st) : launch_append<__nv_bfloat16, 1>(a, st);
+    case kF16: return vec ? launch_append<__half, 16 / sizeof(__half)>(a, st) : launch_append<__half, 1>(a, st);
   }
   return (int)cudaErrorInvalidValue;
 }

@@ -20,8 +20,6 @@ The reference project has no decoding path.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from .. import _native as nat
@@ -30,7 +28,6 @@ from .reference import append_kv_ref, paged_attention_ref
 MAX_HEAD_DIM = 256
 
 _status: dict[int, torch.Tensor] = {}
-_ws_floats: dict[tuple, int] = {}
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
@@ -72,30 +69,42 @@ def _check_cache(k_cache, v_cache, page_table, lengths, like, heads: int, dim: i
 
 
 def _check_no_grad(op: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{op} has no backward pass: call it under torch.no_grad()")
 
 
 def _inner(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if _rows_ok(t) else t.contiguous()
 
 
-def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-              page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None,
-              q: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
-              interleaved: bool = False, force_reference: bool = False) -> torch.Tensor | None:
-    """Store tokens k, v [B, T, Hkv, D] behind each sequence's ``lengths[b]`` cached tokens, in place.
+# What a call's shapes, strides, types and devices (never its addresses) decide: the checks, the array of
+# sizes and strides, the workspace size. A decoding loop repeats them, and checking them anew took longer
+# than the small kernels run.
+_plans: dict[tuple, tuple] = {}
+_MAX_PLANS = 4096
 
-    Token t of sequence b goes to position ``lengths[b] + t``; with ``counts`` [B] int32 only the
-    first ``counts[b]`` of its T tokens are stored (a padded batch; 0 leaves the sequence as it is).
-    With ``cos`` and ``sin`` ([positions, half] fp32, row p for position p) the first ``2 * half``
-    values of each key head, and of each head of ``q`` [B, T, Hq, D], are rotated: value i with
-    value half + i, or with ``interleaved`` neighbours (2i, 2i + 1); in fp32, rounded once.
 
-    Returns q rotated (a new tensor; padding rows too, at most by the tables' last row), a copy of q
-    without tables, or None without q. ``lengths`` is not changed. The slots that one call writes
-    must be distinct.
-    """
+def _keep(key: tuple, plan: tuple) -> tuple:
+    if len(_plans) >= _MAX_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _sig(t: torch.Tensor) -> tuple:
+    return t.shape, t.stride(), t.dtype, t.device
+
+
+def _native(t: torch.Tensor) -> bool:
+    return nat.HAS_NATIVE and t.is_cuda and t.dtype in nat.DT
+
+
+def _rows_ok(*tensors) -> bool:
+    """Whether the kernels read the tensors as they are: unit inner stride."""
+    return all(t is None or t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 for t in tensors)
+
+
+def _append_plan(key, k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved) -> tuple:
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"k and v must both be [B, T, Hkv, D], got {tuple(k.shape)} and {tuple(v.shape)}")
     B, T, Hkv, D = k.shape
@@ -119,33 +128,78 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         raise TypeError(f"counts must be [{B}] int32 on {k.device}")
     if any(n > 1 and s == 0 for c in (k_cache, v_cache) for n, s in zip(c.shape, c.stride())):
         raise ValueError("the cache must not be an expanded tensor: its slots would share memory")
-    _check_no_grad("append_kv", k, v, q, k_cache, v_cache)
-    if force_reference or not (nat.HAS_NATIVE and k.is_cuda and k.dtype in nat.DT):
+    ready = _rows_ok(k, v, page_table, lengths, counts, q) and (
+        cos is None or (cos.is_contiguous() and sin.is_contiguous()))
+    dims = None
+    if ready:
+        Hq, qs = (q.shape[2], q.stride()[:3]) if q is not None else (0, (0, 0, 0))
+        dims = nat.int64s(B, T, Hq, Hkv, D, half, int(interleaved), k_cache.shape[1], k_cache.shape[0],
+                          page_table.shape[1], cos.shape[0] if half else 0, *qs, *k.stride()[:3], *v.stride()[:3],
+                          *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0))
+    return _keep(key, (_native(k), dims))
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None,
+              q: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+              interleaved: bool = False, force_reference: bool = False) -> torch.Tensor | None:
+    """Store tokens k, v [B, T, Hkv, D] behind each sequence's ``lengths[b]`` cached tokens, in place.
+
+    Token t of sequence b goes to position ``lengths[b] + t``; with ``counts`` [B] int32 only the
+    first ``counts[b]`` of its T tokens are stored (a padded batch; 0 leaves the sequence as it is).
+    With ``cos`` and ``sin`` ([positions, half] fp32, row p for position p) the first ``2 * half``
+    values of each key head, and of each head of ``q`` [B, T, Hq, D], are rotated: value i with
+    value half + i, or with ``interleaved`` neighbours (2i, 2i + 1); in fp32, rounded once.
+
+    Returns q rotated (a new tensor; padding rows too, at most by the tables' last row), a copy of q
+    without tables, or None without q. ``lengths`` is not changed. The slots that one call writes
+    must be distinct.
+    """
+    key = (_sig(k), _sig(v), _sig(k_cache), _sig(v_cache), _sig(page_table), _sig(lengths),
+           counts is not None and _sig(counts), q is not None and _sig(q), cos is not None and _sig(cos),
+           sin is not None and _sig(sin), bool(interleaved))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _append_plan(key, k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
+    native, dims = plan
+    if torch.is_grad_enabled():
+        _check_no_grad("append_kv", k, v, q, k_cache, v_cache)
+    if force_reference or not native:
         out = append_kv_ref(k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
         return out.clone() if out is q and q is not None else out
-    k, v = _inner(k), _inner(v)
-    page_table, lengths = _inner(page_table), lengths.contiguous()
-    out = None
-    Hq, qs = 0, (0, 0, 0)
-    if q is not None:
-        q = _inner(q)
-        Hq, qs = q.shape[2], q.stride()[:3]
-        out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    rope_rows = 0
-    if half:
-        cos, sin = cos.contiguous(), sin.contiguous()
-        rope_rows = cos.shape[0]
-    if counts is not None:
-        counts = counts.contiguous()
-    dims = nat.int64s(B, T, Hq, Hkv, D, half, int(interleaved), k_cache.shape[1], k_cache.shape[0],
-                      page_table.shape[1], rope_rows, *qs, *k.stride()[:3], *v.stride()[:3],
-                      *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0))
-    with nat.on_device(k.device):
+    if dims is None:
+        if cos is not None:
+            cos, sin = cos.contiguous(), sin.contiguous()
+        return append_kv(_inner(k), _inner(v), k_cache, v_cache, _inner(page_table), _inner(lengths),
+                         None if counts is None else _inner(counts), None if q is None else _inner(q), cos, sin,
+                         interleaved)
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dev = k.device
+    with nat.on_device(dev):
         nat.call("nfb_append_kv", nat.DT[k.dtype], nat.ptr(q), k.data_ptr(), v.data_ptr(), nat.ptr(out),
                  k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-                 nat.ptr(counts), nat.ptr(cos), nat.ptr(sin), dims, _status_word(k.device).data_ptr(),
-                 nat.stream(k.device))
+                 nat.ptr(counts), nat.ptr(cos), nat.ptr(sin), dims, _status_word(dev).data_ptr(), nat.stream(dev))
     return out
+
+
+def _attention_plan(key, q, k_cache, v_cache, page_table, lengths) -> tuple:
+    if q.dim() != 4 or q.shape[1] != 1:
+        raise ValueError(f"q must be [B, 1, Hq, D], got {tuple(q.shape)}")
+    B, _, Hq, D = q.shape
+    Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
+    _check_cache(k_cache, v_cache, page_table, lengths, q, Hkv, D, B)
+    if Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{Hkv} key heads do not divide {Hq} query heads")
+    if not 0 < D <= MAX_HEAD_DIM:
+        raise ValueError(f"head size {D} is not in 1..{MAX_HEAD_DIM}")
+    native, dims, ws = _native(q), None, 0
+    if native and _rows_ok(q, page_table, lengths):
+        n_pages, ps = k_cache.shape[:2]
+        W = page_table.shape[1]
+        dims = nat.int64s(B, Hq, Hkv, D, ps, n_pages, W, q.stride(0), q.stride(2), Hq * D, D, *k_cache.stride()[:3],
+                          *v_cache.stride()[:3], page_table.stride(0))
+        ws = int(nat.lib().nfb_paged_attn_ws(B, Hq, Hkv, D, ps * W))
+    return _keep(key, (native, dims, ws, D ** -0.5))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -157,35 +211,26 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     defaults to D ** -0.5. A sequence of length 0 answers zeros; what the pages hold behind a
     sequence's length is never used. Statistics and sums are fp32, whatever the cache's type.
     """
-    if q.dim() != 4 or q.shape[1] != 1:
-        raise ValueError(f"q must be [B, 1, Hq, D], got {tuple(q.shape)}")
-    B, _, Hq, D = q.shape
-    Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
-    _check_cache(k_cache, v_cache, page_table, lengths, q, Hkv, D, B)
-    if Hkv < 1 or Hq % Hkv:
-        raise ValueError(f"{Hkv} key heads do not divide {Hq} query heads")
-    if not 0 < D <= MAX_HEAD_DIM:
-        raise ValueError(f"head size {D} is not in 1..{MAX_HEAD_DIM}")
-    _check_no_grad("paged_attention", q, k_cache, v_cache)
-    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    if force_reference or not (nat.HAS_NATIVE and q.is_cuda and q.dtype in nat.DT):
+    key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(page_table), _sig(lengths))
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _attention_plan(key, q, k_cache, v_cache, page_table, lengths)
+    native, dims, n_ws, default = plan
+    if torch.is_grad_enabled():
+        _check_no_grad("paged_attention", q, k_cache, v_cache)
+    sc = default if scale is None else float(scale)
+    if force_reference or not native:
         return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, sc)
-    q = _inner(q)
-    page_table, lengths = _inner(page_table), lengths.contiguous()
-    n_pages, ps = k_cache.shape[:2]
-    W = page_table.shape[1]
-    out = torch.empty((B, 1, Hq, D), dtype=q.dtype, device=q.device)
-    key = (B, Hq, Hkv, D, ps * W)
-    n = _ws_floats.get(key)
-    if n is None:
-        n = _ws_floats[key] = int(nat.lib().nfb_paged_attn_ws(*key))
-    ws = torch.empty(n, dtype=torch.float32, device=q.device)
-    dims = nat.int64s(B, Hq, Hkv, D, ps, n_pages, W, q.stride(0), q.stride(2), Hq * D, D, *k_cache.stride()[:3],
-                      *v_cache.stride()[:3], page_table.stride(0))
-    with nat.on_device(q.device):
+    if dims is None:
+        return paged_attention(_inner(q), k_cache, v_cache, _inner(page_table), _inner(lengths), sc)
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    # the caching allocator's memory, new for each call: calls on other streams and in other graphs have theirs
+    ws = torch.empty(n_ws, dtype=torch.float32, device=dev).data_ptr() if n_ws else None
+    with nat.on_device(dev):
         nat.call("nfb_paged_attn", nat.DT[q.dtype], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                 page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), ws.data_ptr(), dims, sc,
-                 _status_word(q.device).data_ptr(), nat.stream(q.device))
+                 page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), ws, dims, sc,
+                 _status_word(dev).data_ptr(), nat.stream(dev))
     return out
 
 
