@@ -10,13 +10,17 @@
 // Sums and statistics are fp32; m and s are kept apart for the backward pass (their sum m + log s
 // would round away the low bits of log s).
 #include <climits>
+#include <cooperative_groups.h>
 
 #include "common.cuh"
 
 namespace nfb {
 
+namespace cg = cooperative_groups;
+
 enum LogprobSite : uint32_t { kSiteTarget = 1 };
 constexpr int kMaxTop = 32;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct LpArgs {
   const void* logits;
@@ -26,54 +30,261 @@ struct LpArgs {
   int64_t* top_tokens;
   uint32_t* status;
   int64_t rows, ld, ignore_index;
-  int V, top_k;
+  int V, top_k, split;  // split: CTAs (one cluster) a row
 };
 
 struct Stat { float m, s, u; };  // u: sum of exp(z - m) (z - m)
 
-// (x - m) clamped so that a masked logit gives 0 * finite, not 0 * inf; NaN passes through.
+// (z - m) clamped so that a masked logit gives 0 * finite, not 0 * inf; NaN passes through.
 __device__ __forceinline__ float clamp_low(float d) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-1e4f));
   return r;
 }
+__device__ __forceinline__ float exp_of(float d) {  // 2^-22 relative, of a difference that is exact or nearly so
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * kLog2e));
+  return y;
+}
+__device__ __forceinline__ float or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
+// `a` moved to the maximum m: exp(z - m) (z - m) = exp(d) exp(z - a.m) ((z - a.m) + d), d = a.m - m.
+__device__ __forceinline__ Stat stat_at(Stat a, float m) {
+  const float d = clamp_low(a.m - or_zero(m)), e = exp_of(d);
+  return {m, a.s * e, e * (a.u + a.s * d)};
+}
 __device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
   const float m = fmaxf(a.m, b.m);
-  const float base = m == -INFINITY ? 0.f : m;
-  const float da = clamp_low(a.m - base), db = clamp_low(b.m - base);
-  const float ea = expf(da), eb = expf(db);
-  // exp(z - m) (z - m) = exp(d) exp(z - m') ((z - m') + d) for m = m' - d
-  return {m, a.s * ea + b.s * eb, ea * (a.u + a.s * da) + eb * (b.u + b.s * db)};
+  a = stat_at(a, m);
+  b = stat_at(b, m);
+  return {m, a.s + b.s, a.u + b.u};
 }
 
+// Order of the alternatives as one number: the value (zeros of both signs alike), then the lower index.
+__device__ __forceinline__ uint64_t rank_key(float z, int j) {
+  const uint32_t b = __float_as_uint(z + 0.f);
+  return (uint64_t)(b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (uint32_t)~j;
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __uint_as_float(b ^ ((b >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Forward. A CTA (or a cluster of them, where there are few rows) has a row and takes it in segments
+// of up to 64 KB, held in its threads' registers: each thread finds its own maximum and sums its
+// exponentials against that, so the row is read once and no thread waits for a common maximum.
+//
+// Alternatives: the k-th largest of the maxima of 32 groups of 16 threads bounds the k-th largest
+// logit from below, so only threads whose own maximum reaches it look at their values again; the few
+// candidates (about k) are ranked against one another. Rows with so many equal values that the
+// candidates overflow take k rounds of a block-wide maximum instead. One warp finds the bound while
+// the others sum. Later segments start from the best of the earlier ones.
+//
+// What bounds it: 2 bytes a value at the HBM's rate need one exponential for each 1.4 clocks of an
+// SM quarter's special-function unit; the loads of one CTA run while the other's exponentials do.
+constexpr int kLpThreads = 512, kLpVecs = 8, kLpWarps = kLpThreads / 32, kLpCand = 512;
+
 template <typename T>
-__global__ void __launch_bounds__(512) logprobs_kernel(const LpArgs a) {
-  __shared__ Stat red[16];
-  __shared__ float red_v[16];
-  __shared__ int red_i[16];
-  __shared__ float best_v;
-  __shared__ int best_i;
-  const int64_t row = blockIdx.x;
+__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a) {
+  constexpr int VE = 16 / sizeof(T);
+  __shared__ Stat s_stat[kLpWarps];
+  __shared__ float s_group[32];
+  __shared__ float s_bound;
+  __shared__ int s_count;
+  __shared__ uint64_t s_cand[kLpCand];
+  __shared__ uint64_t s_top[2][kMaxTop];  // keys of the best so far, descending; 0: none
+  __shared__ uint64_t s_round[kLpWarps];
+  __shared__ Stat s_part;
+  __shared__ uint64_t s_best[kMaxTop];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t row = a.split == 1 ? blockIdx.x : blockIdx.x / a.split;
+  const int rank = a.split == 1 ? 0 : blockIdx.x % a.split;
   const T* x = (const T*)a.logits + row * a.ld;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  Stat st{-INFINITY, 0.f, 0.f};
-  for (int j = threadIdx.x; j < a.V; j += blockDim.x) {
-    const float z = to_f32(x[j]);
-    // the element's own statistics: NaN must reach the sums, so s is exp(z - z) rather than 1
-    const float d = clamp_low(z - (z == -INFINITY ? 0.f : z));
-    st = stat_merge(st, Stat{z, expf(d), 0.f});
+  const int k = a.top_k;
+  // rows begin anywhere: values in front of the first 16-byte boundary and behind the last one are
+  // taken one by one by the first threads
+  const int head = min(a.V, (int)((-reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)));
+  const int vecs = (a.V - head) / VE, tail = head + vecs * VE;
+  const int per = (vecs + a.split - 1) / a.split;
+  const int first = min(vecs, rank * per), last = min(vecs, first + per);
+  int extra = -1;  // index of this thread's single value
+  if (rank == 0) {
+    if (tid < head) extra = tid;
+    else if (tid - head < a.V - tail) extra = tail + (tid - head);
   }
+  Stat st{-INFINITY, 0.f, 0.f};
+  int top = 0;  // which of s_top holds the best so far
+  if (k > 0 && tid < kMaxTop) s_top[0][tid] = 0;
+  if (tid == 0) s_count = 0;
+  for (int base = first; base == first || base < last; base += kLpThreads * kLpVecs) {
+    uint4 d[kLpVecs];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    st = stat_merge(st, Stat{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                             __shfl_xor_sync(0xffffffffu, st.u, o)});
-  if (lane == 0) red[warp] = st;
+    for (int i = 0; i < kLpVecs; ++i) {
+      const int v = base + i * kLpThreads + tid;
+      const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+      d[i] = make_uint4(none, none, none, none);  // -inf
+      if (v < last) d[i] = __ldcs(reinterpret_cast<const uint4*>(x + head) + v);
+    }
+    const float ex = base == first && extra >= 0 ? to_f32(x[extra]) : -INFINITY;
+    float mx = ex;
+#pragma unroll
+    for (int i = 0; i < kLpVecs; ++i) {
+      float z[VE];
+      unpack16<T>(d[i], z);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) mx = fmaxf(mx, z[e]);
+    }
+    if (k > 0) {
+      float g = mx;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((lane & 15) == 0) s_group[tid >> 4] = g;
+      __syncthreads();
+      if (warp == 0) {
+        g = s_group[lane];
+        int better = 0;
+#pragma unroll
+        for (int o = 1; o < 32; ++o) {
+          const float v = __shfl_sync(0xffffffffu, g, (lane + o) & 31);
+          better += v > g || (v == g && ((lane + o) & 31) < lane);
+        }
+        if (better == k - 1) {
+          const uint64_t kth = s_top[top][k - 1];
+          s_bound = kth != 0 ? fmaxf(g, key_value(kth)) : g;
+        }
+        if (lane == 0) s_count = 0;
+      }
+    }
+    // this thread's sums, against its own maximum
+    if (mx > st.m) st = stat_at(st, mx);
+    const float m = or_zero(st.m);
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int i = 0; i < kLpVecs; ++i) {
+      float z[VE];
+      unpack16<T>(d[i], z);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float df = clamp_low(z[e] - m), p = exp_of(df);
+        s += p;
+        u = fmaf(p, df, u);
+      }
+    }
+    {
+      const float df = clamp_low(ex - m), p = exp_of(df);
+      s += p;
+      u = fmaf(p, df, u);
+    }
+    st.s += s;
+    st.u += u;
+    if (k > 0) {
+      __syncthreads();
+      const float bound = s_bound;
+      auto each = [&](auto&& f) {  // this thread's values with their indices
+        if (base == first && extra >= 0) f(ex, extra);
+#pragma unroll
+        for (int i = 0; i < kLpVecs; ++i) {
+          const int v = base + i * kLpThreads + tid;
+          if (v >= last) break;
+          float z[VE];
+          unpack16<T>(d[i], z);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) f(z[e], head + v * VE + e);
+        }
+      };
+      if (mx >= bound) {
+        each([&](float z, int j) {
+          if (z >= bound) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kLpCand) s_cand[at] = rank_key(z, j);
+          }
+        });
+      }
+      if (base != first && tid < k && s_top[top][tid] != 0) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kLpCand) s_cand[at] = s_top[top][tid];
+      }
+      if (tid < kMaxTop) s_top[top ^ 1][tid] = 0;
+      __syncthreads();
+      const int n = s_count;
+      if (n <= kLpCand) {
+        if (tid < n) {
+          const uint64_t mine = s_cand[tid];
+          int better = 0;
+          for (int i = 0; i < n; ++i) better += s_cand[i] > mine;
+          if (better < k) s_top[top ^ 1][better] = mine;
+        }
+      } else {
+        uint64_t below = ~0ull;
+        for (int r = 0; r < k; ++r) {
+          uint64_t best = base != first && tid < k && s_top[top][tid] < below ? s_top[top][tid] : 0;
+          each([&](float z, int j) {
+            const uint64_t key = rank_key(z, j);
+            if (z == z && key < below && key > best) best = key;
+          });
+          best = warp_max_key(best);
+          if (lane == 0) s_round[warp] = best;
+          __syncthreads();
+          best = s_round[lane & (kLpWarps - 1)];
+          best = warp_max_key(best);
+          if (tid == 0) s_top[top ^ 1][r] = best;
+          below = best;
+          __syncthreads();
+        }
+      }
+      top ^= 1;
+    }
+  }
+  // the row's statistics: warps, then the block
+  float m = warp_max(st.m);
+  st = stat_at(st, m);
+  st.s = warp_sum(st.s);
+  st.u = warp_sum(st.u);
+  if (lane == 0) s_stat[warp] = st;
   __syncthreads();
-  st = red[0];
-  for (int w = 1; w < warps; ++w) st = stat_merge(st, red[w]);
-  const float m = st.m == -INFINITY ? 0.f : st.m, log_s = logf(st.s);
-  if (threadIdx.x == 0) {
+  if (warp == 0) {
+    st = s_stat[lane & (kLpWarps - 1)];
+    m = warp_max(st.m);
+    st = stat_at(st, m);
+    if (lane >= kLpWarps) st.s = st.u = 0.f;
+    st.s = warp_sum(st.s);
+    st.u = warp_sum(st.u);
+  }
+  if (a.split > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) s_part = st;
+    if (tid < k) s_best[tid] = s_top[top][tid];
+    cluster.sync();
+    if (rank == 0 && warp == 0) {
+      for (int r = 1; r < a.split; ++r) st = stat_merge(st, *cluster.map_shared_rank(&s_part, r));
+      if (k > 0) {  // the CTAs' lists, ranked again
+        __syncwarp();
+        for (int r = 0; r < a.split; ++r)
+          if (lane < k) s_cand[r * k + lane] = cluster.map_shared_rank(s_best, r)[lane];
+        if (lane < k) s_top[top ^ 1][lane] = 0;
+        __syncwarp();
+        for (int i = lane; i < a.split * k; i += 32) {
+          const uint64_t mine = s_cand[i];
+          int better = 0;
+          for (int o = 0; o < a.split * k; ++o) better += s_cand[o] > mine;
+          if (mine != 0 && better < k) s_top[top ^ 1][better] = mine;
+        }
+        __syncwarp();
+        top ^= 1;
+      }
+    }
+    cluster.sync();  // the other CTAs' shared memory has been read
+    if (rank != 0) return;
+  }
+  if (warp != 0) return;
+  m = or_zero(st.m);
+  const float log_s = logf(st.s);
+  if (lane == 0) {
     a.stats[2 * row] = m;
     a.stats[2 * row + 1] = st.s;
     // a row without a finite logit has no distribution: its entropy is 0
@@ -86,43 +297,16 @@ __global__ void __launch_bounds__(512) logprobs_kernel(const LpArgs a) {
           set_status(a.status, kBadArgument, kSiteTarget);
           lp = __int_as_float(0x7fffffff);
         } else {
-          const float z = to_f32(x[t]);
-          lp = st.s == 0.f ? -INFINITY : (z - m) - log_s;
+          lp = st.s == 0.f ? -INFINITY : (to_f32(x[t]) - m) - log_s;
         }
       }
       a.logprobs[row] = lp;
     }
   }
-  // top_k rounds of the largest (value, lowest index) behind the last one
-  float last_v = INFINITY;
-  int last_i = -1;
-  for (int k = 0; k < a.top_k; ++k) {
-    float bv = -INFINITY;
-    int bi = INT_MAX;
-    for (int j = threadIdx.x; j < a.V; j += blockDim.x) {
-      const float z = to_f32(x[j]);
-      const bool behind = z < last_v || (z == last_v && j > last_i);
-      if (behind && (z > bv || (z == bv && j < bi))) { bv = z; bi = j; }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float v = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int i = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (v > bv || (v == bv && i < bi)) { bv = v; bi = i; }
-    }
-    if (lane == 0) { red_v[warp] = bv; red_i[warp] = bi; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < warps; ++w)
-        if (red_v[w] > bv || (red_v[w] == bv && red_i[w] < bi)) { bv = red_v[w]; bi = red_i[w]; }
-      best_v = bv;
-      best_i = bi;
-      a.top_tokens[row * a.top_k + k] = bi == INT_MAX ? 0 : bi;  // only rows with NaN run out of values
-      a.top_logprobs[row * a.top_k + k] = st.s == 0.f ? -INFINITY : (bv - m) - log_s;
-    }
-    __syncthreads();
-    last_v = best_v;
-    last_i = best_i;
+  if (lane < k) {
+    const uint64_t key = s_top[top][lane];  // 0: only a row with NaN runs out of values
+    a.top_tokens[row * k + lane] = key == 0 ? 0 : (int)~(uint32_t)key;
+    a.top_logprobs[row * k + lane] = st.s == 0.f ? -INFINITY : (key_value(key) - m) - log_s;
   }
 }
 
@@ -133,24 +317,33 @@ struct LpBwdArgs {
   const float *stats, *entropy;
   void* d_logits;
   int64_t rows, ld, ignore_index;
-  int V, top_k;
+  int V, top_k, chunks, per;  // CTAs a row; values of a chunk
 };
 
-template <typename T>
-__global__ void __launch_bounds__(512) logprobs_bwd_kernel(const LpBwdArgs a) {
+// Backward: a stream over the row, bound by its bytes (each logit read, each gradient written). With
+// d = z - m the gradient apart from the given tokens is exp(d) (c1 d + c0), c0 and c1 of the row. The
+// given tokens' places are written again by the first threads, each with its whole value (a token may
+// be the target and an alternative), rounded once.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) logprobs_bwd_kernel(const LpBwdArgs a) {
+  constexpr int VE = 16 / sizeof(T), kVecs = 4;
   __shared__ int s_idx[kMaxTop + 1];
   __shared__ float s_g[kMaxTop + 1];
-  const int64_t row = blockIdx.x;
+  const int64_t row = blockIdx.x / a.chunks;
+  const int chunk = (int)(blockIdx.x - row * a.chunks);
   const T* x = (const T*)a.logits + row * a.ld;
   T* dx = (T*)a.d_logits + row * a.V;
   const int n_fix = a.top_k + 1;
-  if (threadIdx.x < n_fix) {  // entry 0: the target; then the alternatives
+  if ((int)threadIdx.x < n_fix) {  // entry 0: the target; then the alternatives
     int j = -1;
     float g = 0.f;
     if (threadIdx.x == 0) {
-      if (a.g_logprobs && a.targets[row] != a.ignore_index && a.targets[row] >= 0 && a.targets[row] < a.V) {
-        j = (int)a.targets[row];
-        g = a.g_logprobs[row];
+      if (a.g_logprobs) {
+        const int64_t t = a.targets[row];
+        if (t != a.ignore_index && t >= 0 && t < a.V) {
+          j = (int)t;
+          g = a.g_logprobs[row];
+        }
       }
     } else if (a.g_top) {
       j = (int)a.top_tokens[row * a.top_k + threadIdx.x - 1];
@@ -159,20 +352,54 @@ __global__ void __launch_bounds__(512) logprobs_bwd_kernel(const LpBwdArgs a) {
     s_idx[threadIdx.x] = j;
     s_g[threadIdx.x] = g;
   }
-  __syncthreads();
-  float whole = 0.f;
-  for (int i = 0; i < n_fix; ++i) whole += s_g[i];
   const float m = a.stats[2 * row], s = a.stats[2 * row + 1], log_s = logf(s);
   const float e = a.g_entropy ? a.g_entropy[row] : 0.f, H = a.entropy[row];
   const float inv = s == 0.f ? 0.f : 1.f / s;
-  for (int j = threadIdx.x; j < a.V; j += blockDim.x) {
-    const float d = clamp_low(to_f32(x[j]) - m);
-    const float p = s == 0.f ? 0.f : expf(d) * inv;
-    float g = s == 0.f ? 0.f : -p * (whole + e * ((d - log_s) + H));
-    if (s != 0.f)
-      for (int i = 0; i < n_fix; ++i)
-        if (s_idx[i] == j) g += s_g[i];
-    dx[j] = from_f32<T>(g);
+  __syncthreads();
+  float whole = 0.f;
+  for (int i = 0; i < n_fix; ++i) whole += s_g[i];
+  // a row without a finite logit has s = 0: no gradient
+  const float c0 = s == 0.f ? 0.f : -(whole + e * (H - log_s)) * inv, c1 = -e * inv;
+  auto grad = [&](float z) {
+    const float d = clamp_low(z - m);
+    return exp_of(d) * fmaf(c1, d, c0);
+  };
+  const int begin = chunk * a.per, end = min(a.V, begin + a.per);
+  if constexpr (VEC) {
+    // x and dx begin at the same distance from a 16-byte boundary
+    const int head = min(end, begin + (int)((-reinterpret_cast<uintptr_t>(x + begin) & 15) / sizeof(T)));
+    const int vecs = (end - head) / VE, tail = head + vecs * VE;
+    if ((int)threadIdx.x < head - begin) dx[begin + threadIdx.x] = from_f32<T>(grad(to_f32(x[begin + threadIdx.x])));
+    if ((int)threadIdx.x < end - tail) dx[tail + threadIdx.x] = from_f32<T>(grad(to_f32(x[tail + threadIdx.x])));
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+    uint4* dv = reinterpret_cast<uint4*>(dx + head);
+    for (int v0 = threadIdx.x; v0 < vecs; v0 += kVecs * 256) {
+      uint4 w[kVecs];
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        if (v0 + i * 256 < vecs) w[i] = __ldcs(xv + v0 + i * 256);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) {
+        if (v0 + i * 256 < vecs) {
+          float z[VE];
+          unpack16<T>(w[i], z);
+#pragma unroll
+          for (int k = 0; k < VE; ++k) z[k] = grad(z[k]);
+          dv[v0 + i * 256] = pack16<T>(z);
+        }
+      }
+    }
+  } else {
+    for (int j = begin + threadIdx.x; j < end; j += 256) dx[j] = from_f32<T>(grad(to_f32(x[j])));
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < n_fix && s != 0.f) {
+    const int j = s_idx[threadIdx.x];
+    if (j >= begin && j < end) {
+      float g = 0.f;
+      for (int i = 0; i < n_fix; ++i) g += s_idx[i] == j ? s_g[i] : 0.f;
+      dx[j] = from_f32<T>(g + grad(to_f32(x[j])));
+    }
   }
 }
 
@@ -180,20 +407,60 @@ __global__ void __launch_bounds__(512) logprobs_bwd_kernel(const LpBwdArgs a) {
 
 using namespace nfb;
 
+namespace {
+
+template <typename T>
+int launch_fwd(LpArgs& a, cudaStream_t st) {
+  // a cluster for each row while the rows do not fill the GPU and each CTA keeps a vector a thread
+  const int slots = 2 * nfb_num_sms();
+  const int64_t vecs = a.V / (int64_t)(16 / sizeof(T));
+  a.split = 1;
+  while (a.split < 8 && a.rows * a.split * 2 <= slots && vecs >= (int64_t)a.split * 2 * kLpThreads) a.split *= 2;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)a.split;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * a.split));
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+}
+
+template <typename T>
+int launch_bwd(LpBwdArgs& a, cudaStream_t st) {
+  constexpr int kChunk = 256 * 4 * 16 / sizeof(T);  // one round of every thread's vectors
+  a.chunks = (int)(((int64_t)a.V + kChunk - 1) / kChunk);
+  // chunks of whole 16-byte pieces and of like size
+  a.per = (int)((((int64_t)a.V + a.chunks - 1) / a.chunks + 7) / 8 * 8);
+  if (a.rows * a.chunks > INT_MAX) return (int)cudaErrorInvalidValue;
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.d_logits)) & 15) == 0 &&
+                   (a.ld - a.V) * (int64_t)sizeof(T) % 16 == 0;
+  const unsigned grid = (unsigned)(a.rows * a.chunks);
+  if (vec) logprobs_bwd_kernel<T, true><<<grid, 256, 0, st>>>(a);
+  else logprobs_bwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace
+
 NFB_API int nfb_logprobs_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V, const int64_t* targets,
                              int64_t ignore_index, int top_k, float* logprobs, float* entropy, float* stats,
                              float* top_logprobs, int64_t* top_tokens, uint32_t* status, void* stream) {
   if (rows == 0) return 0;
-  if (rows < 0 || rows > INT_MAX || V < 1 || V > INT_MAX - 4096 || top_k < 0 || top_k > kMaxTop || top_k > V)
+  if (rows < 0 || rows > INT_MAX || V < 1 || V > INT_MAX - (1 << 20) || top_k < 0 || top_k > kMaxTop || top_k > V)
     return (int)cudaErrorInvalidValue;
-  const LpArgs a{logits, targets, logprobs, entropy, stats, top_logprobs, top_tokens, status,
-                 rows, ld, ignore_index, (int)V, top_k};
+  LpArgs a{logits, targets, logprobs, entropy, stats, top_logprobs, top_tokens, status,
+           rows, ld, ignore_index, (int)V, top_k, 1};
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == kF32) logprobs_kernel<float><<<(unsigned)rows, 512, 0, st>>>(a);
-  else if (dtype == kBF16) logprobs_kernel<__nv_bfloat16><<<(unsigned)rows, 512, 0, st>>>(a);
-  else if (dtype == kF16) logprobs_kernel<__half><<<(unsigned)rows, 512, 0, st>>>(a);
-  else return (int)cudaErrorInvalidValue;
-  return (int)cudaGetLastError();
+  switch (dtype) {
+    case kF32: return launch_fwd<float>(a, st);
+    case kBF16: return launch_fwd<__nv_bfloat16>(a, st);
+    case kF16: return launch_fwd<__half>(a, st);
+  }
+  return (int)cudaErrorInvalidValue;
 }
 
 NFB_API int nfb_logprobs_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V, const int64_t* targets,
@@ -201,14 +468,15 @@ NFB_API int nfb_logprobs_bwd(int dtype, const void* logits, int64_t ld, int64_t 
                              const float* g_entropy, const float* g_top, const float* stats, const float* entropy,
                              void* d_logits, void* stream) {
   if (rows == 0) return 0;
-  if (rows < 0 || rows > INT_MAX || V < 1 || V > INT_MAX - 4096 || top_k < 0 || top_k > kMaxTop || top_k > V)
+  if (rows < 0 || rows > INT_MAX || V < 1 || V > INT_MAX - (1 << 20) || top_k < 0 || top_k > kMaxTop || top_k > V)
     return (int)cudaErrorInvalidValue;
-  const LpBwdArgs a{logits, targets, top_tokens, g_logprobs, g_entropy, g_top, stats, entropy, d_logits,
-                    rows, ld, ignore_index, (int)V, top_k};
+  LpBwdArgs a{logits, targets, top_tokens, g_logprobs, g_entropy, g_top, stats, entropy, d_logits,
+              rows, ld, ignore_index, (int)V, top_k, 1, 0};
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == kF32) logprobs_bwd_kernel<float><<<(unsigned)rows, 512, 0, st>>>(a);
-  else if (dtype == kBF16) logprobs_bwd_kernel<__nv_bfloat16><<<(unsigned)rows, 512, 0, st>>>(a);
-  else if (dtype == kF16) logprobs_bwd_kernel<__half><<<(unsigned)rows, 512, 0, st>>>(a);
-  else return (int)cudaErrorInvalidValue;
-  return (int)cudaGetLastError();
+  switch (dtype) {
+    case kF32: return launch_bwd<float>(a, st);
+    case kBF16: return launch_bwd<__nv_bfloat16>(a, st);
+    case kF16: return launch_bwd<__half>(a, st);
+  }
+  return (int)cudaErrorInvalidValue;
 }

@@ -292,12 +292,15 @@ def test_rows_past_32_bits():
     t[-3:] = t3
     leaf = x.requires_grad_(True)
     r = token_logprobs(leaf, t, top_k=2)
-    small = y.clone().requires_grad_(True)
-    e = token_logprobs(small, t3, top_k=2)
-    assert torch.equal(r.logprobs[-3:], e.logprobs) and torch.equal(r.top_tokens[-3:], e.top_tokens)
+    one, none = torch.ones(3, device=DEV), torch.zeros(3, device=DEV)
+    ref = _plain64(y, t3, 2, -100, one, none, torch.zeros(3, 2, device=DEV))
+    # against the definition, not against a call of three rows: that one divides each row over several
+    # blocks, so its sums are added in another order and either is within the tolerance of the exact value
+    _close(r.logprobs[-3:].detach(), ref["given"], ref["ts"] + 2.0 ** -22 * (ref["given"].abs() + math.log(V) + 1))
+    assert torch.equal(r.top_tokens[-3:], ref["ids"])
     (dx,) = torch.autograd.grad(r.logprobs.sum(), leaf)
-    (de,) = torch.autograd.grad(e.logprobs.sum(), small)
-    assert torch.equal(dx[-3:], de) and not dx[:-3].any()
+    _close(dx[-3:], ref["dx"], torch.finfo(torch.bfloat16).eps / 2 * ref["dx"].abs() + ref["tol_dx"] * (1 + 2 ** -7) + 2.0 ** -126)
+    assert not dx[:-3].any()
 
 
 def test_repeats_are_bit_identical_and_native():
