@@ -7,8 +7,8 @@
 // nothing to either sum. The alternatives are the top_k largest logits, equal ones in the order of
 // their index. The gradient of g log p_t + e H + sum_i a_i log p_{k_i} is
 //   dz_j = -p_j (g + sum_i a_i + e (log p_j + H)) + g [j = t] + sum_i a_i [j = k_i].
-// Sums and statistics are fp32; m and s are kept apart for the backward pass (their sum m + log s
-// would round away the low bits of log s).
+// Sums and statistics are fp32; m and s are kept apart for the backward pass, since their sum
+// m + log s would round away the low bits of log s.
 #include <climits>
 #include <cooperative_groups.h>
 
@@ -25,7 +25,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 struct LpArgs {
   const void* logits;
   const int64_t* targets;  // null: none
-  float *logprobs, *entropy, *stats;  // stats: (m, s) per row
+  float *logprobs, *entropy, *stats;  // stats: (m, s) of each row
   float* top_logprobs;
   int64_t* top_tokens;
   uint32_t* status;
@@ -33,25 +33,26 @@ struct LpArgs {
   int V, top_k, split;  // split: CTAs (one cluster) a row
 };
 
-struct Stat { float m, s, u; };  // u: sum of exp(z - m) (z - m)
+struct Stat { float m, s, u; };  // maximum; sums of exp(z - m) and of exp(z - m) (z - m)
 
-// (z - m) clamped so that a masked logit gives 0 * finite, not 0 * inf; NaN passes through.
-__device__ __forceinline__ float clamp_low(float d) {
+// z - m clamped so that a masked logit gives 0 * finite, not 0 * inf; NaN passes through. (The
+// difference is taken before the factor log2(e): a row at the type's lowest value stays finite.)
+__device__ __forceinline__ float below_max(float z, float m) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-1e4f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z - m), "f"(-1e4f));
   return r;
 }
-__device__ __forceinline__ float exp_of(float d) {  // 2^-22 relative, of a difference that is exact or nearly so
+__device__ __forceinline__ float exp_of(float d) {  // 2^-22 relative
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * kLog2e));
   return y;
 }
 __device__ __forceinline__ float or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// `a` moved to the maximum m: exp(z - m) (z - m) = exp(d) exp(z - a.m) ((z - a.m) + d), d = a.m - m.
+// `a` moved to the maximum m: exp(d + c) (d + c) with c = a.m - m.
 __device__ __forceinline__ Stat stat_at(Stat a, float m) {
-  const float d = clamp_low(a.m - or_zero(m)), e = exp_of(d);
-  return {m, a.s * e, e * (a.u + a.s * d)};
+  const float c = below_max(a.m, or_zero(m)), e = exp_of(c);
+  return {m, a.s * e, e * (a.u + a.s * c)};
 }
 __device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
   const float m = fmaxf(a.m, b.m);
@@ -75,32 +76,45 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// Forward. A CTA (or a cluster of them, where there are few rows) has a row and takes it in segments
-// of up to 64 KB, held in its threads' registers: each thread finds its own maximum and sums its
-// exponentials against that, so the row is read once and no thread waits for a common maximum.
-//
-// Alternatives: the k-th largest of the maxima of 32 groups of 16 threads bounds the k-th largest
-// logit from below, so only threads whose own maximum reaches it look at their values again; the few
-// candidates (about k) are ranked against one another. Rows with so many equal values that the
-// candidates overflow take k rounds of a block-wide maximum instead. One warp finds the bound while
-// the others sum. Later segments start from the best of the earlier ones.
-//
-// What bounds it: 2 bytes a value at the HBM's rate need one exponential for each 1.4 clocks of an
-// SM quarter's special-function unit; the loads of one CTA run while the other's exponentials do.
-constexpr int kLpThreads = 512, kLpVecs = 8, kLpWarps = kLpThreads / 32, kLpCand = 512;
-
+// Largest of a 16-byte vector's values, NaN left out; pairs of 16-bit values at a time.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a) {
-  constexpr int VE = 16 / sizeof(T);
-  __shared__ Stat s_stat[kLpWarps];
+__device__ __forceinline__ float vec_max(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(&v);
+    const T2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(to_f32(m.x), to_f32(m.y));
+  }
+}
+
+// Forward. A CTA (or a cluster of them, where there are few rows) streams over a row: each thread
+// keeps sums against its own running maximum, so the row is read once, no thread waits for a common
+// maximum, and few registers leave room for the loads of many rows in flight.
+//
+// Alternatives: the k-th largest of the maxima of 32 groups of threads bounds the k-th largest logit
+// from below, so only threads whose own maximum reaches the bound read their values again (from the
+// L2); the few candidates (about k) are ranked against one another. If values equal to the bound
+// overflow the candidates (a constant or fully masked row), those above it are ranked and the first
+// ones equal to it taken in the order of the row; if even the greater ones overflow (sorted rows),
+// k rounds of a block-wide maximum remain.
+//
+// What bounds it: 2 bytes a value at the HBM's rate leave 1.4 clocks of an SM quarter's
+// special-function unit for each exponential, which takes 0.25 to 0.5 of that.
+constexpr int kLpUnroll = 4, kLpAbove = 1024, kLpEqual = 256;
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a) {
+  constexpr int VE = 16 / sizeof(T), kWarps = NT / 32, kGroup = NT / 32;  // 32 groups of kGroup threads
+  __shared__ Stat s_stat[kWarps];
   __shared__ float s_group[32];
   __shared__ float s_bound;
-  __shared__ int s_count;
-  __shared__ uint64_t s_cand[kLpCand];
-  __shared__ uint64_t s_top[2][kMaxTop];  // keys of the best so far, descending; 0: none
-  __shared__ uint64_t s_round[kLpWarps];
-  __shared__ Stat s_part;
-  __shared__ uint64_t s_best[kMaxTop];
+  __shared__ int s_above, s_equal;            // candidates above the bound and equal to it
+  __shared__ uint64_t s_cand[kLpAbove + kLpEqual];
+  __shared__ uint64_t s_best[kMaxTop];        // keys of the alternatives, descending; 0: none
+  __shared__ uint64_t s_round[kWarps];
+  __shared__ Stat s_row;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = a.split == 1 ? blockIdx.x : blockIdx.x / a.split;
   const int rank = a.split == 1 ? 0 : blockIdx.x % a.split;
@@ -109,204 +123,225 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const LpArgs a)
   // rows begin anywhere: values in front of the first 16-byte boundary and behind the last one are
   // taken one by one by the first threads
   const int head = min(a.V, (int)((-reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)));
-  const int vecs = (a.V - head) / VE, tail = head + vecs * VE;
+  const int vecs = (a.V - head) / VE;
   const int per = (vecs + a.split - 1) / a.split;
   const int first = min(vecs, rank * per), last = min(vecs, first + per);
-  int extra = -1;  // index of this thread's single value
-  if (rank == 0) {
-    if (tid < head) extra = tid;
-    else if (tid - head < a.V - tail) extra = tail + (tid - head);
-  }
+  const int lo = rank == 0 ? 0 : head + first * VE, hi = rank == a.split - 1 ? a.V : head + last * VE;
+  const int n_front = head + first * VE - lo, n_back = hi - (head + last * VE);
+  const int single = tid < n_front ? lo + tid : tid - n_front < n_back ? head + last * VE + (tid - n_front) : -1;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+  if (tid < kMaxTop) s_best[tid] = 0;
+  if (tid == 0) s_above = s_equal = 0;
+
+  float mx = single >= 0 ? to_f32(x[single]) : -INFINITY;
   Stat st{-INFINITY, 0.f, 0.f};
-  int top = 0;  // which of s_top holds the best so far
-  if (k > 0 && tid < kMaxTop) s_top[0][tid] = 0;
-  if (tid == 0) s_count = 0;
-  for (int base = first; base == first || base < last; base += kLpThreads * kLpVecs) {
-    uint4 d[kLpVecs];
+  {
+    const float z = mx;
+    st.m = mx = fmaxf(mx, -INFINITY);  // NaN left out
+    const float d = below_max(z, or_zero(mx));
+    if (single >= 0) {
+      st.s = exp_of(d);
+      st.u = st.s * d;
+    }
+  }
+  for (int v0 = first + tid; v0 < last; v0 += NT * kLpUnroll) {
+    uint4 w[kLpUnroll];
 #pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) {
-      const int v = base + i * kLpThreads + tid;
+    for (int i = 0; i < kLpUnroll; ++i) {
       const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
-      d[i] = make_uint4(none, none, none, none);  // -inf
-      if (v < last) d[i] = __ldcs(reinterpret_cast<const uint4*>(x + head) + v);
+      w[i] = make_uint4(none, none, none, none);  // -inf
+      if (v0 + i * NT < last) w[i] = __ldg(xv + v0 + i * NT);
     }
-    const float ex = base == first && extra >= 0 ? to_f32(x[extra]) : -INFINITY;
-    float mx = ex;
+    float m = vec_max<T>(w[0]);
 #pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) {
-      float z[VE];
-      unpack16<T>(d[i], z);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) mx = fmaxf(mx, z[e]);
+    for (int i = 1; i < kLpUnroll; ++i) m = fmaxf(m, vec_max<T>(w[i]));
+    if (m > mx) {
+      mx = m;
+      st = stat_at(st, mx);
     }
-    if (k > 0) {
-      float g = mx;
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-      if ((lane & 15) == 0) s_group[tid >> 4] = g;
-      __syncthreads();
-      if (warp == 0) {
-        g = s_group[lane];
-        int better = 0;
-#pragma unroll
-        for (int o = 1; o < 32; ++o) {
-          const float v = __shfl_sync(0xffffffffu, g, (lane + o) & 31);
-          better += v > g || (v == g && ((lane + o) & 31) < lane);
-        }
-        if (better == k - 1) {
-          const uint64_t kth = s_top[top][k - 1];
-          s_bound = kth != 0 ? fmaxf(g, key_value(kth)) : g;
-        }
-        if (lane == 0) s_count = 0;
-      }
-    }
-    // this thread's sums, against its own maximum
-    if (mx > st.m) st = stat_at(st, mx);
-    const float m = or_zero(st.m);
+    const float base = or_zero(mx);
     float s = 0.f, u = 0.f;
 #pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) {
+    for (int i = 0; i < kLpUnroll; ++i) {
       float z[VE];
-      unpack16<T>(d[i], z);
+      unpack16<T>(w[i], z);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float df = clamp_low(z[e] - m), p = exp_of(df);
+        const float d = below_max(z[e], base), p = exp_of(d);
         s += p;
-        u = fmaf(p, df, u);
+        u = fmaf(p, d, u);
       }
-    }
-    {
-      const float df = clamp_low(ex - m), p = exp_of(df);
-      s += p;
-      u = fmaf(p, df, u);
     }
     st.s += s;
     st.u += u;
-    if (k > 0) {
-      __syncthreads();
-      const float bound = s_bound;
-      auto each = [&](auto&& f) {  // this thread's values with their indices
-        if (base == first && extra >= 0) f(ex, extra);
+  }
+  // the warps' sums, then the row's by warp 1 while warp 0 looks for the bound
+  {
+    Stat t = stat_at(st, warp_max(st.m));
+    t.s = warp_sum(t.s);
+    t.u = warp_sum(t.u);
+    if (lane == 0) s_stat[warp] = t;
+  }
+  if (k > 0) {
+    float g = mx;
 #pragma unroll
-        for (int i = 0; i < kLpVecs; ++i) {
-          const int v = base + i * kLpThreads + tid;
-          if (v >= last) break;
-          float z[VE];
-          unpack16<T>(d[i], z);
+    for (int o = kGroup / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (lane % kGroup == 0) s_group[tid / kGroup] = g;
+  }
+  __syncthreads();
+  if (warp == 1) {
+    Stat t = lane < kWarps ? s_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+    t = stat_at(t, warp_max(t.m));
+    t.s = warp_sum(t.s);
+    t.u = warp_sum(t.u);
+    if (lane == 0) s_row = t;
+  }
+  if (k > 0) {
+    if (warp == 0) {
+      const float g = s_group[lane];
+      int better = 0;
 #pragma unroll
-          for (int e = 0; e < VE; ++e) f(z[e], head + v * VE + e);
+      for (int o = 1; o < 32; ++o) {
+        const float v = __shfl_sync(0xffffffffu, g, (lane + o) & 31);
+        better += v > g || (v == g && ((lane + o) & 31) < lane);
+      }
+      if (better == k - 1) s_bound = g;
+    }
+    __syncthreads();
+    const float bound = s_bound;
+    if (mx >= bound) {
+      auto take = [&](float z, int j) {
+        if (z > bound) {
+          const int at = atomicAdd(&s_above, 1);
+          if (at < kLpAbove) s_cand[at] = rank_key(z, j);
+        } else if (z == bound) {
+          const int at = atomicAdd(&s_equal, 1);
+          if (at < kLpEqual) s_cand[kLpAbove + at] = rank_key(z, j);
         }
       };
-      if (mx >= bound) {
-        each([&](float z, int j) {
-          if (z >= bound) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kLpCand) s_cand[at] = rank_key(z, j);
-          }
-        });
-      }
-      if (base != first && tid < k && s_top[top][tid] != 0) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kLpCand) s_cand[at] = s_top[top][tid];
-      }
-      if (tid < kMaxTop) s_top[top ^ 1][tid] = 0;
-      __syncthreads();
-      const int n = s_count;
-      if (n <= kLpCand) {
-        if (tid < n) {
-          const uint64_t mine = s_cand[tid];
-          int better = 0;
-          for (int i = 0; i < n; ++i) better += s_cand[i] > mine;
-          if (better < k) s_top[top ^ 1][better] = mine;
-        }
-      } else {
-        uint64_t below = ~0ull;
-        for (int r = 0; r < k; ++r) {
-          uint64_t best = base != first && tid < k && s_top[top][tid] < below ? s_top[top][tid] : 0;
-          each([&](float z, int j) {
-            const uint64_t key = rank_key(z, j);
-            if (z == z && key < below && key > best) best = key;
-          });
-          best = warp_max_key(best);
-          if (lane == 0) s_round[warp] = best;
-          __syncthreads();
-          best = s_round[lane & (kLpWarps - 1)];
-          best = warp_max_key(best);
-          if (tid == 0) s_top[top ^ 1][r] = best;
-          below = best;
-          __syncthreads();
+      if (single >= 0) take(to_f32(x[single]), single);
+#pragma unroll 4
+      for (int v = first + tid; v < last; v += NT) {
+        const uint4 w = __ldg(xv + v);
+        if (vec_max<T>(w) >= bound) {
+          float z[VE];
+          unpack16<T>(w, z);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) take(z[e], head + v * VE + e);
         }
       }
-      top ^= 1;
+    }
+    __syncthreads();
+    const int above = s_above, equal = s_equal;
+    if (above >= k ? above <= kLpAbove : equal <= kLpEqual) {
+      // rank those above the bound, and those equal to it where they are needed
+      const int n = above >= k ? above : above + equal;
+      for (int i = tid; i < n; i += NT) {
+        const uint64_t mine = s_cand[i < above ? i : kLpAbove + (i - above)];
+        int better = 0;
+        for (int o = 0; o < above; ++o) better += s_cand[o] > mine;
+        if (i >= above)
+          for (int o = 0; o < equal; ++o) better += s_cand[kLpAbove + o] > mine;
+        if (better < k) s_best[better] = mine;
+      }
+    } else if (above < k) {
+      if (tid < above) {
+        const uint64_t mine = s_cand[tid];
+        int better = 0;
+        for (int o = 0; o < above; ++o) better += s_cand[o] > mine;
+        s_best[better] = mine;
+      }
+      int found = above;  // the first equal ones in the order of the row
+      for (int j0 = lo; j0 < hi && found < k; j0 += NT) {
+        const int j = j0 + tid;
+        const float z = j < hi ? to_f32(x[j]) : 0.f;
+        const uint32_t hit = __ballot_sync(0xffffffffu, j < hi && z == bound);
+        if (lane == 0) s_round[warp] = __popc(hit);
+        __syncthreads();
+        int at = found;
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) at += (int)s_round[w];
+          found += (int)s_round[w];
+        }
+        at += __popc(hit & ((1u << lane) - 1));
+        if ((hit >> lane & 1) && at < k) s_best[at] = rank_key(z, j);
+        __syncthreads();
+      }
+    } else {
+      uint64_t below = ~0ull;
+      for (int r = 0; r < k; ++r) {
+        uint64_t best = 0;
+        auto look = [&](float z, int j) {
+          const uint64_t key = rank_key(z, j);
+          if (z == z && key < below && key > best) best = key;
+        };
+        if (single >= 0) look(to_f32(x[single]), single);
+        for (int v = first + tid; v < last; v += NT) {
+          float z[VE];
+          unpack16<T>(__ldg(xv + v), z);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) look(z[e], head + v * VE + e);
+        }
+        best = warp_max_key(best);
+        if (lane == 0) s_round[warp] = best;
+        __syncthreads();
+        best = warp_max_key(lane < kWarps ? s_round[lane] : 0);
+        if (tid == 0) s_best[r] = best;
+        below = best;
+        __syncthreads();
+      }
     }
   }
-  // the row's statistics: warps, then the block
-  float m = warp_max(st.m);
-  st = stat_at(st, m);
-  st.s = warp_sum(st.s);
-  st.u = warp_sum(st.u);
-  if (lane == 0) s_stat[warp] = st;
   __syncthreads();
-  if (warp == 0) {
-    st = s_stat[lane & (kLpWarps - 1)];
-    m = warp_max(st.m);
-    st = stat_at(st, m);
-    if (lane >= kLpWarps) st.s = st.u = 0.f;
-    st.s = warp_sum(st.s);
-    st.u = warp_sum(st.u);
-  }
+  Stat t = s_row;
   if (a.split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
-    if (tid == 0) s_part = st;
-    if (tid < k) s_best[tid] = s_top[top][tid];
     cluster.sync();
     if (rank == 0 && warp == 0) {
-      for (int r = 1; r < a.split; ++r) st = stat_merge(st, *cluster.map_shared_rank(&s_part, r));
+      for (int r = 1; r < a.split; ++r) t = stat_merge(t, *cluster.map_shared_rank(&s_row, r));
       if (k > 0) {  // the CTAs' lists, ranked again
-        __syncwarp();
         for (int r = 0; r < a.split; ++r)
           if (lane < k) s_cand[r * k + lane] = cluster.map_shared_rank(s_best, r)[lane];
-        if (lane < k) s_top[top ^ 1][lane] = 0;
+        __syncwarp();
+        if (lane < k) s_best[lane] = 0;
         __syncwarp();
         for (int i = lane; i < a.split * k; i += 32) {
           const uint64_t mine = s_cand[i];
           int better = 0;
           for (int o = 0; o < a.split * k; ++o) better += s_cand[o] > mine;
-          if (mine != 0 && better < k) s_top[top ^ 1][better] = mine;
+          if (mine != 0 && better < k) s_best[better] = mine;
         }
         __syncwarp();
-        top ^= 1;
       }
     }
     cluster.sync();  // the other CTAs' shared memory has been read
     if (rank != 0) return;
   }
   if (warp != 0) return;
-  m = or_zero(st.m);
-  const float log_s = logf(st.s);
+  const float m = or_zero(t.m), log_s = logf(t.s);
   if (lane == 0) {
     a.stats[2 * row] = m;
-    a.stats[2 * row + 1] = st.s;
+    a.stats[2 * row + 1] = t.s;
     // a row without a finite logit has no distribution: its entropy is 0
-    a.entropy[row] = st.s == 0.f ? 0.f : log_s - st.u / st.s;
+    a.entropy[row] = t.s == 0.f ? 0.f : log_s - t.u / t.s;
     if (a.targets) {
-      const int64_t t = a.targets[row];
+      const int64_t j = a.targets[row];
       float lp = 0.f;
-      if (t != a.ignore_index) {
-        if (t < 0 || t >= a.V) {
+      if (j != a.ignore_index) {
+        if (j < 0 || j >= a.V) {
           set_status(a.status, kBadArgument, kSiteTarget);
           lp = __int_as_float(0x7fffffff);
         } else {
-          lp = st.s == 0.f ? -INFINITY : (to_f32(x[t]) - m) - log_s;
+          lp = t.s == 0.f ? -INFINITY : (to_f32(x[j]) - m) - log_s;
         }
       }
       a.logprobs[row] = lp;
     }
   }
   if (lane < k) {
-    const uint64_t key = s_top[top][lane];  // 0: only a row with NaN runs out of values
+    const uint64_t key = s_best[lane];  // 0: only a row with NaN runs out of values
     a.top_tokens[row * k + lane] = key == 0 ? 0 : (int)~(uint32_t)key;
-    a.top_logprobs[row * k + lane] = st.s == 0.f ? -INFINITY : (key_value(key) - m) - log_s;
+    a.top_logprobs[row * k + lane] = t.s == 0.f ? -INFINITY : (key_value(key) - m) - log_s;
   }
 }
 
@@ -361,7 +396,7 @@ __global__ void __launch_bounds__(256) logprobs_bwd_kernel(const LpBwdArgs a) {
   // a row without a finite logit has s = 0: no gradient
   const float c0 = s == 0.f ? 0.f : -(whole + e * (H - log_s)) * inv, c1 = -e * inv;
   auto grad = [&](float z) {
-    const float d = clamp_low(z - m);
+    const float d = below_max(z, m);
     return exp_of(d) * fmaf(c1, d, c0);
   };
   const int begin = chunk * a.per, end = min(a.V, begin + a.per);
@@ -409,24 +444,29 @@ using namespace nfb;
 
 namespace {
 
-template <typename T>
-int launch_fwd(LpArgs& a, cudaStream_t st) {
-  // a cluster for each row while the rows do not fill the GPU and each CTA keeps a vector a thread
-  const int slots = 2 * nfb_num_sms();
+template <typename T, int NT>
+int launch_fwd_nt(LpArgs& a, cudaStream_t st) {
+  // a cluster for each row while the rows leave SMs idle and each CTA keeps two vectors a thread
   const int64_t vecs = a.V / (int64_t)(16 / sizeof(T));
   a.split = 1;
-  while (a.split < 8 && a.rows * a.split * 2 <= slots && vecs >= (int64_t)a.split * 2 * kLpThreads) a.split *= 2;
+  while (a.split < 8 && a.rows * a.split * 2 <= 2 * nfb_num_sms() && vecs >= (int64_t)a.split * 4 * NT) a.split *= 2;
+  if (a.rows * a.split > INT_MAX) return (int)cudaErrorInvalidValue;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = (unsigned)a.split;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * a.split));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(NT);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = a.split > 1 ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+  return (int)cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT>, a);
+}
+
+template <typename T>
+int launch_fwd(LpArgs& a, cudaStream_t st) {
+  return a.V * (int64_t)sizeof(T) < 16384 ? launch_fwd_nt<T, 128>(a, st) : launch_fwd_nt<T, 256>(a, st);
 }
 
 template <typename T>
