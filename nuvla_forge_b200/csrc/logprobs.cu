@@ -25,7 +25,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 struct LpArgs {
   const void* logits;
   const int64_t* targets;  // null: none
-  float *logprobs, *entropy, *stats;  // stats: (m, s) of each row
+  float *logprobs, *entropy, *stats;  // stats: (m, s) of each row, or null
   float* top_logprobs;
   int64_t* top_tokens;
   uint32_t* status;
@@ -89,16 +89,46 @@ __device__ __forceinline__ float vec_max(const uint4& v) {
   }
 }
 
+// The row is read once here, so it leaves no lines in L1; it stays in the L2 for a backward pass.
+__device__ __forceinline__ uint4 ld_row(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// The k-th largest of the warp's 32 values (counted with repetition).
+__device__ __forceinline__ float kth_of_warp(float v, int k) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  const uint32_t key = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  bool in = true;
+  uint32_t best = 0;
+  if (k <= 16) {
+    for (int i = 0; i < k; ++i) {  // the largest one leaves
+      best = __reduce_max_sync(0xffffffffu, in ? key : 0u);
+      const uint32_t who = __ballot_sync(0xffffffffu, in && key == best);
+      in = in && (int)(threadIdx.x & 31) != __ffs(who) - 1;
+    }
+  } else {
+    for (int i = k; i <= 32; ++i) {  // the smallest one leaves
+      best = __reduce_min_sync(0xffffffffu, in ? key : 0xFFFFFFFFu);
+      const uint32_t who = __ballot_sync(0xffffffffu, in && key == best);
+      in = in && (int)(threadIdx.x & 31) != __ffs(who) - 1;
+    }
+  }
+  return __uint_as_float(best ^ ((best >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
 // Forward. A CTA (or a cluster of them, where there are few rows) streams over a row: each thread
 // keeps sums against its own running maximum, so the row is read once, no thread waits for a common
 // maximum, and few registers leave room for the loads of many rows in flight.
 //
 // Alternatives: the k-th largest of the maxima of 32 groups of threads bounds the k-th largest logit
-// from below, so only threads whose own maximum reaches the bound read their values again (from the
-// L2); the few candidates (about k) are ranked against one another. If values equal to the bound
-// overflow the candidates (a constant or fully masked row), those above it are ranked and the first
-// ones equal to it taken in the order of the row; if even the greater ones overflow (sorted rows),
-// k rounds of a block-wide maximum remain.
+// from below. The bound is taken after every thread's first vectors and renewed as the row goes by (a
+// group maximum that is read late is only a lower bound, so nobody waits); values that reach it are
+// put aside, some k (1 + log(row / first vectors)) of them, and ranked at the end. Where more come
+// (a rising row, a constant or fully masked one) the row is looked at again: with the final bound,
+// those above it are ranked and the first ones equal to it taken in the order of the row; if even the
+// greater ones overflow (a sorted row), k rounds of a block-wide maximum remain.
 //
 // What bounds it: 2 bytes a value at the HBM's rate leave 1.4 clocks of an SM quarter's
 // special-function unit for each exponential, which takes 0.25 to 0.5 of that.
@@ -109,8 +139,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
   constexpr int VE = 16 / sizeof(T), kWarps = NT / 32, kGroup = NT / 32;  // 32 groups of kGroup threads
   __shared__ Stat s_stat[kWarps];
   __shared__ float s_group[32];
-  __shared__ float s_bound;
-  __shared__ int s_above, s_equal;            // candidates above the bound and equal to it
+  __shared__ int s_above, s_equal;            // values put aside (first look: all of them in s_above)
   __shared__ uint64_t s_cand[kLpAbove + kLpEqual];
   __shared__ uint64_t s_best[kMaxTop];        // keys of the alternatives, descending; 0: none
   __shared__ uint64_t s_round[kWarps];
@@ -144,22 +173,59 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
       st.u = st.s * d;
     }
   }
-  for (int v0 = first + tid; v0 < last; v0 += NT * kLpUnroll) {
+  float bound = INFINITY;
+  volatile float* group = s_group;
+  auto publish = [&](float m) {  // this thread's group maximum so far
+#pragma unroll
+    for (int o = kGroup / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane % kGroup == 0) group[tid / kGroup] = m;
+  };
+  auto aside = [&](float z, int j) {
+    if (z >= bound) {
+      const int at = atomicAdd(&s_above, 1);
+      if (at < kLpAbove) s_cand[at] = rank_key(z, j);
+    }
+  };
+  int turn = 0;
+  for (int base = first; base == first || base < last; base += NT * kLpUnroll, ++turn) {
+    const int v0 = base + tid;
     uint4 w[kLpUnroll];
 #pragma unroll
     for (int i = 0; i < kLpUnroll; ++i) {
       const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
       w[i] = make_uint4(none, none, none, none);  // -inf
-      if (v0 + i * NT < last) w[i] = __ldg(xv + v0 + i * NT);
+      if (v0 + i * NT < last) w[i] = ld_row(xv + v0 + i * NT);
     }
-    float m = vec_max<T>(w[0]);
+    float vm[kLpUnroll], m = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < kLpUnroll; ++i) m = fmaxf(m, vec_max<T>(w[i]));
+    for (int i = 0; i < kLpUnroll; ++i) {
+      vm[i] = vec_max<T>(w[i]);
+      m = fmaxf(m, vm[i]);
+    }
     if (m > mx) {
       mx = m;
       st = stat_at(st, mx);
     }
-    const float base = or_zero(mx);
+    if (k > 0) {
+      if ((turn & (turn - 1)) == 0) {  // the first vectors, and at 1, 2, 4, ... times as many
+        publish(mx);
+        if (turn == 0) __syncthreads();
+        bound = kth_of_warp(group[lane], k);
+        if (turn == 0 && single >= 0) aside(to_f32(x[single]), single);
+      }
+      if (m >= bound) {
+#pragma unroll
+        for (int i = 0; i < kLpUnroll; ++i) {
+          if (vm[i] >= bound && v0 + i * NT < last) {
+            float z[VE];
+            unpack16<T>(w[i], z);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) aside(z[e], head + (v0 + i * NT) * VE + e);
+          }
+        }
+      }
+    }
+    const float ref = or_zero(mx);
     float s = 0.f, u = 0.f;
 #pragma unroll
     for (int i = 0; i < kLpUnroll; ++i) {
@@ -167,7 +233,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
       unpack16<T>(w[i], z);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float d = below_max(z[e], base), p = exp_of(d);
+        const float d = below_max(z[e], ref), p = exp_of(d);
         s += p;
         u = fmaf(p, d, u);
       }
@@ -175,19 +241,14 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     st.s += s;
     st.u += u;
   }
-  // the warps' sums, then the row's by warp 1 while warp 0 looks for the bound
+  // the warps' sums, then the row's by warp 1 while the others rank
   {
     Stat t = stat_at(st, warp_max(st.m));
     t.s = warp_sum(t.s);
     t.u = warp_sum(t.u);
     if (lane == 0) s_stat[warp] = t;
   }
-  if (k > 0) {
-    float g = mx;
-#pragma unroll
-    for (int o = kGroup / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (lane % kGroup == 0) s_group[tid / kGroup] = g;
-  }
+  if (k > 0) publish(mx);
   __syncthreads();
   if (warp == 1) {
     Stat t = lane < kWarps ? s_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
@@ -196,19 +257,33 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     t.u = warp_sum(t.u);
     if (lane == 0) s_row = t;
   }
-  if (k > 0) {
-    if (warp == 0) {
-      const float g = s_group[lane];
-      int better = 0;
+  const int put = k > 0 ? s_above : 0;
+  auto rank_in = [&](const uint64_t* list, int n, uint64_t mine) {
+    int better = 0;
+    for (int o = 0; o < n; ++o) better += list[o] > mine;
+    if (better < k) s_best[better] = mine;
+  };
+  if (put <= 192) {
+    for (int i = tid; i < put; i += NT) rank_in(s_cand, put, s_cand[i]);
+  } else if (put <= kLpAbove) {
+    // many: those that the final bound leaves first, since ranking costs the square
+    bound = kth_of_warp(group[lane], k);
+    uint64_t mine[kLpAbove / NT];
 #pragma unroll
-      for (int o = 1; o < 32; ++o) {
-        const float v = __shfl_sync(0xffffffffu, g, (lane + o) & 31);
-        better += v > g || (v == g && ((lane + o) & 31) < lane);
-      }
-      if (better == k - 1) s_bound = g;
-    }
+    for (int i = 0; i < kLpAbove / NT; ++i) mine[i] = tid + i * NT < put ? s_cand[tid + i * NT] : 0;
     __syncthreads();
-    const float bound = s_bound;
+    const uint64_t least = rank_key(bound, -1);  // behind every index: below all keys of its value
+#pragma unroll
+    for (int i = 0; i < kLpAbove / NT; ++i)
+      if (mine[i] >= least) s_cand[atomicAdd(&s_equal, 1)] = mine[i];
+    __syncthreads();
+    const int left = s_equal;
+    for (int i = tid; i < left; i += NT) rank_in(s_cand, left, s_cand[i]);
+  } else {
+    bound = kth_of_warp(group[lane], k);
+    __syncthreads();
+    if (tid == 0) s_above = s_equal = 0;
+    __syncthreads();
     if (mx >= bound) {
       auto take = [&](float z, int j) {
         if (z > bound) {
@@ -245,12 +320,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
         if (better < k) s_best[better] = mine;
       }
     } else if (above < k) {
-      if (tid < above) {
-        const uint64_t mine = s_cand[tid];
-        int better = 0;
-        for (int o = 0; o < above; ++o) better += s_cand[o] > mine;
-        s_best[better] = mine;
-      }
+      if (tid < above) rank_in(s_cand, above, s_cand[tid]);
       int found = above;  // the first equal ones in the order of the row
       for (int j0 = lo; j0 < hi && found < k; j0 += NT) {
         const int j = j0 + tid;
@@ -320,8 +390,10 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
   if (warp != 0) return;
   const float m = or_zero(t.m), log_s = logf(t.s);
   if (lane == 0) {
-    a.stats[2 * row] = m;
-    a.stats[2 * row + 1] = t.s;
+    if (a.stats) {
+      a.stats[2 * row] = m;
+      a.stats[2 * row + 1] = t.s;
+    }
     // a row without a finite logit has no distribution: its entropy is 0
     a.entropy[row] = t.s == 0.f ? 0.f : log_s - t.u / t.s;
     if (a.targets) {
@@ -464,9 +536,15 @@ int launch_fwd_nt(LpArgs& a, cudaStream_t st) {
   return (int)cudaLaunchKernelEx(&cfg, logprobs_kernel<T, NT>, a);
 }
 
+// Threads a row: few for short rows and where many rows fill the GPU anyway (less waiting for one
+// another: 16384 x 32000 bf16 with 5 alternatives 234 us with 128, 257 us with 256; 20000 x 2000 fp16
+// 48 us with 64, 66 us with 128), many for few rows (64 x 32000 bf16: 7.4 us with 256, 8.7 us with 128).
 template <typename T>
 int launch_fwd(LpArgs& a, cudaStream_t st) {
-  return a.V * (int64_t)sizeof(T) < 16384 ? launch_fwd_nt<T, 128>(a, st) : launch_fwd_nt<T, 256>(a, st);
+  const int64_t bytes = a.V * (int64_t)sizeof(T);
+  if (bytes < 8192) return launch_fwd_nt<T, 64>(a, st);
+  if (bytes < 16384 || a.rows >= 12 * (int64_t)nfb_num_sms()) return launch_fwd_nt<T, 128>(a, st);
+  return launch_fwd_nt<T, 256>(a, st);
 }
 
 template <typename T>

@@ -52,15 +52,15 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, x, targets, top_k, ignore_index):
         M, V = x.shape
         dev = x.device
-        f32 = dict(dtype=torch.float32, device=dev)
-        logprobs = torch.empty(M, **f32) if targets is not None else None
-        entropy = torch.empty(M, **f32)
-        stats = torch.empty((M, 2), **f32)
-        top = torch.empty((M, top_k), **f32) if top_k else None
+        f32 = torch.float32
+        logprobs = torch.empty(M, dtype=f32, device=dev) if targets is not None else None
+        entropy = torch.empty(M, dtype=f32, device=dev)
+        stats = torch.empty((M, 2), dtype=f32, device=dev) if ctx is not None else None  # for the backward pass
+        top = torch.empty((M, top_k), dtype=f32, device=dev) if top_k else None
         ids = torch.empty((M, top_k), dtype=torch.int64, device=dev) if top_k else None
         with nat.on_device(dev):
             nat.call("nfb_logprobs_fwd", nat.DT[x.dtype], x.data_ptr(), x.stride(0), M, V, nat.ptr(targets),
-                     ignore_index, top_k, nat.ptr(logprobs), entropy.data_ptr(), stats.data_ptr(), nat.ptr(top),
+                     ignore_index, top_k, nat.ptr(logprobs), entropy.data_ptr(), nat.ptr(stats), nat.ptr(top),
                      nat.ptr(ids), _status_word(dev).data_ptr(), nat.stream(dev))
         if ctx is not None:
             ctx.set_materialize_grads(False)
@@ -112,8 +112,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
             raise ValueError(f"targets must be {tuple(lead)} on {logits.device}, got {tuple(targets.shape)} on "
                              f"{targets.device}")
     top_k, ignore_index = int(top_k), int(ignore_index)
-    x = logits.reshape(-1, V)
-    t = None if targets is None else targets.reshape(-1)
+    flat = len(lead) == 1
+    x = logits if flat else logits.reshape(-1, V)
+    t = targets if flat or targets is None else targets.reshape(-1)
     if force_reference or not (nat.HAS_NATIVE and x.is_cuda and x.dtype in nat.DT):
         r = token_logprobs_ref(x, t, top_k, ignore_index)
     else:
@@ -124,7 +125,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
             r = _TokenLogprobs.apply(x, t, top_k, ignore_index)
         else:
             r = _TokenLogprobs.forward(None, x, t, top_k, ignore_index)
-    if len(lead) == 1:
+    if flat:
         return TokenLogprobs(*r)
     lp, h, top, ids = r
     return TokenLogprobs(None if lp is None else lp.view(lead), h.view(lead),
