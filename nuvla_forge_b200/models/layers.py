@@ -29,7 +29,7 @@ import torch.utils.checkpoint
 import torch.nn.functional as F
 from torch import nn
 
-from ..ops import add_rmsnorm
+from ..ops import add_rmsnorm, append_kv, paged_attention
 from ..ops import attention as attention_op
 from ..ops import linear as linear_op
 from ..ops import rmsnorm as rmsnorm_op
@@ -105,6 +105,55 @@ class TimestepEmbedder(nn.Module):
         return linear(h, l2.weight, l2.bias)
 
 
+class PagedKVCache:
+    """Keys and values of a stack of blocks in pages, for decoding one token at a time.
+
+    Every layer has pools [n_pages, page_size, Hkv, D]; one ``page_table`` [B, W] and one ``lengths``
+    [B] (tokens stored so far) serve all layers. A forward pass over new tokens runs between
+    ``begin(t, counts)`` and ``advance()``: in it each layer stores its t tokens (the first
+    ``counts[b]`` of them) behind ``lengths`` and attends over ``seen`` = lengths + stored tokens.
+    """
+
+    def __init__(self, n_layers: int, batch_size: int, max_len: int, kv_heads: int, head_dim: int,
+                 page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cpu"):
+        per = -(-max_len // page_size)
+        shape = (batch_size * per, page_size, kv_heads, head_dim)
+        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        self.page_table = torch.arange(batch_size * per, dtype=torch.int32, device=device).view(batch_size, per)
+        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        self.seen = torch.zeros_like(self.lengths)
+        self.max_len = max_len
+        self.counts: torch.Tensor | None = None
+
+    def layer(self, i: int) -> "CacheLayer":
+        return CacheLayer(self, i)
+
+    def begin(self, tokens: int, counts: torch.Tensor | None = None) -> None:
+        self.counts = counts
+        torch.add(self.lengths, tokens if counts is None else counts, out=self.seen)
+
+    def advance(self) -> None:
+        self.lengths.copy_(self.seen)
+
+    def reset(self) -> None:
+        self.lengths.zero_()
+
+
+class CacheLayer:
+    """One layer of a :class:`PagedKVCache`."""
+
+    def __init__(self, cache: PagedKVCache, i: int):
+        self.cache, self.k, self.v = cache, cache.k[i], cache.v[i]
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        c = self.cache
+        append_kv(k, v, self.k, self.v, c.page_table, c.lengths, c.counts)
+
+    def attend(self, q: torch.Tensor) -> torch.Tensor:
+        return paged_attention(q, self.k, self.v, self.cache.page_table, self.cache.seen)
+
+
 class Attention(nn.Module):
     """Multi-head / grouped-query attention with a fused qkv projection.
 
@@ -132,7 +181,9 @@ class Attention(nn.Module):
             self.qkv = nn.Linear(dim, dim + 2 * kvd, bias=False)
         self.proj = nn.Linear(dim, dim, bias=False)
 
-    def forward(self, x, context=None, residual=None):
+    def forward(self, x, context=None, residual=None, cache: CacheLayer | None = None):
+        """``cache``: also store this call's keys and values; a single token attends over the stored
+        ones (its own included), several tokens over one another (they begin their sequences)."""
         b, t, c = x.shape
         H, Hk, Dh = self.n_heads, self.kv_heads, self.head_dim
         if context is None:
@@ -147,7 +198,12 @@ class Attention(nn.Module):
                 q = linear(x, self.qkv.weight[:c]).view(b, t, H, Dh)
                 kv = linear(context, self.qkv.weight[c:]).view(b, s, 2 * Hk, Dh)
             k, v = kv.split([Hk, Hk], dim=2)
-        o = attention_op(q, k, v, causal=self.causal and context is None, force_reference=not self.fused)
+        if cache is not None:
+            cache.append(k, v)
+        if cache is not None and t == 1:
+            o = cache.attend(q)
+        else:
+            o = attention_op(q, k, v, causal=self.causal and context is None, force_reference=not self.fused)
         o = o.reshape(b, t, c)
         return _linear(o, self.proj.weight, residual=residual)
 
@@ -249,32 +305,39 @@ class TransformerBlock(nn.Module):
         x = self.attn(self.norm1(x), residual=x)
         return self.mlp(self.norm2(x), residual=x)
 
-    def forward_chain(self, x, pending=None):
+    def forward_chain(self, x, pending=None, cache: CacheLayer | None = None):
         """Same block with every residual add folded into the following RMSNorm kernel.
 
         ``pending`` is the previous block's MLP output not yet added to ``x``.
         Returns (x, this block's MLP output, not yet added).
         """
+        if cache is not None:
+            return self._chain(x, pending, cache)
         return checkpointed(self, self._chain, x, pending)
 
-    def _chain(self, x, pending):
+    def _chain(self, x, pending, cache: CacheLayer | None = None):
         ref = not self.norm1.fused
         if pending is None:
             h = self.norm1(x)
         else:
             x, h = add_rmsnorm(x, pending, self.norm1.weight, self.norm1.eps, force_reference=ref)
-        x, h = add_rmsnorm(x, self.attn(h), self.norm2.weight, self.norm2.eps, force_reference=ref)
+        a = self.attn(h) if cache is None else self.attn(h, cache=cache)
+        x, h = add_rmsnorm(x, a, self.norm2.weight, self.norm2.eps, force_reference=ref)
         return x, self.mlp(h)
 
 
-def run_blocks(blocks, x, final_norm: RMSNorm | None = None):
+def run_blocks(blocks, x, final_norm: RMSNorm | None = None, cache: PagedKVCache | None = None):
     """Run a stack of TransformerBlocks with residual adds fused into the norms.
 
-    Returns final_norm(x_out) when ``final_norm`` is given, else x_out.
+    Returns final_norm(x_out) when ``final_norm`` is given, else x_out. With ``cache`` every block's
+    keys and values are stored (between the cache's ``begin`` and ``advance``).
     """
     pending = None
-    for blk in blocks:
-        x, pending = blk.forward_chain(x, pending)
+    for i, blk in enumerate(blocks):
+        if cache is None:
+            x, pending = blk.forward_chain(x, pending)
+        else:
+            x, pending = blk.forward_chain(x, pending, cache.layer(i))
     if pending is None:
         return final_norm(x) if final_norm is not None else x
     if final_norm is None:

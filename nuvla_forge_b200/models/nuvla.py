@@ -37,11 +37,11 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from ..ops import chunked_cross_entropy, patchify_images
+from ..ops import TokenLogprobs, chunked_cross_entropy, patchify_images, token_logprobs
 from ..ops import attention as attention_op
 from ..ops.image import patch_kpad
 from .dit import TrajectoryDiT
-from .layers import RMSNorm, TransformerBlock, _linear, linear, run_blocks
+from .layers import PagedKVCache, RMSNorm, TransformerBlock, _linear, linear, run_blocks
 
 
 @dataclass
@@ -336,6 +336,55 @@ class NuVLA(nn.Module):
     def plan(self, images, text_tokens=None, steps: int = 10, z0: torch.Tensor | None = None):
         """Sample waypoints [B, horizon, traj_dim] by Euler integration of the DiT's velocity."""
         return self.dit.sample(self.context(images, text_tokens), steps=steps, z0=z0)
+
+    # -- answering with the reasoning head (BASELINE layout) ---------------
+    def _needs_causal_backbone(self) -> None:
+        if not self.cfg.backbone_over_images:
+            raise ValueError("answering needs the causal backbone over images and text (backbone_over_images); the "
+                             "reference layout's text branch sees all of its tokens at once")
+
+    def score_text(self, images, text_tokens, text_targets, top_k: int = 0, ignore_index: int = -100) -> TokenLogprobs:
+        """Log probabilities [B, T] of ``text_targets`` under the reasoning head, each position's entropy and its
+        ``top_k`` most likely tokens; differentiable (``ops.token_logprobs``)."""
+        self._needs_causal_backbone()
+        img = self.image_tokens(images)
+        txt = self.text_embed(text_tokens) + self.text_pos[:, : text_tokens.shape[1]]
+        h = run_blocks(self.text_blocks, torch.cat([img, txt.to(img.dtype)], dim=1), self.text_norm)
+        return token_logprobs(self.text_logits(h[:, img.shape[1]:]), text_targets, top_k=top_k,
+                              ignore_index=ignore_index, force_reference=not self.cfg.fused)
+
+    def text_logits(self, h):
+        return linear(h, self.lm_head)
+
+    def new_cache(self, batch_size: int, max_len: int, page_size: int = 64) -> PagedKVCache:
+        """An empty cache for ``max_len`` image and text tokens of each sequence."""
+        self._needs_causal_backbone()
+        attn = self.text_blocks[0].attn
+        p = self.lm_head
+        return PagedKVCache(len(self.text_blocks), batch_size, max_len, attn.kv_heads, attn.head_dim, page_size,
+                            p.dtype, p.device)
+
+    @torch.no_grad()
+    def read_prompt(self, images, text_tokens, cache: PagedKVCache):
+        """Backbone states [B, L, D] of images and instruction; their keys and values fill the empty ``cache``."""
+        img = self.image_tokens(images)
+        txt = self.text_embed(text_tokens) + self.text_pos[:, : text_tokens.shape[1]]
+        h = torch.cat([img, txt.to(img.dtype)], dim=1)
+        cache.reset()
+        cache.begin(h.shape[1])
+        h = run_blocks(self.text_blocks, h, self.text_norm, cache=cache)
+        cache.advance()
+        return h
+
+    @torch.no_grad()
+    def read_token(self, tokens, text_position, cache: PagedKVCache, counts=None):
+        """Backbone states [B, 1, D] of one more token [B] each; ``text_position`` is an int64 tensor [1], ``counts``
+        [B] int32 (0: this sequence is finished and is not stored)."""
+        h = self.text_embed(tokens)[:, None] + self.text_pos[:, text_position]
+        cache.begin(1, counts)
+        h = run_blocks(self.text_blocks, h.to(self.lm_head.dtype), self.text_norm, cache=cache)
+        cache.advance()
+        return h
 
     def num_parameters(self) -> int:
         return sum(p.numel() for p in self.parameters())
