@@ -190,6 +190,8 @@ __global__ void __launch_bounds__(kAppendThreads, 12) append_kernel(const Append
 // ---------------------------------------------------------------------------------------------
 constexpr int kTile = 16;
 constexpr int kAttnWarps = 4;
+// Resident CTAs an SM of the tensor-core kernel, by its registers.
+__host__ __device__ constexpr int attn_ctas(int D, int NG) { return NG > 1 ? 2 : D <= 64 ? 4 : 3; }
 
 struct AttnArgs {
   const void *q, *k_cache, *v_cache;
@@ -200,94 +202,97 @@ struct AttnArgs {
   int B, Hq, Hkv, D, G;        // G = Hq / Hkv query heads per key head
   int rows, subs, units;       // query heads a unit covers; units per key head; units per sequence
   int whole;                   // one CTA for each (sequence, unit): nothing is shared
-  int ctas, min_tiles;
+  int ctas, big, min_tiles;    // CTAs, and how many of them take the larger runs
+  float share;                 // of the list that those take
+  int cap;                     // tokens that a row of the table has room for
   int page_size, n_pages, table_width;
   int64_t q_sb, q_sh, o_sb, o_sh, kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh, t_sb;
   float scale_log2;            // scale * log2(e): exponentials are taken to base 2
 };
 
 __device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
-  const int64_t cap = min((int64_t)a.table_width * a.page_size, (int64_t)INT_MAX - 2 * kTile);
   int n = a.lengths[b];
-  if (n < 0 || n > cap) {
+  if (n < 0 || n > a.cap) {
     set_status(a.status, kBadArgument, kSiteAttnLen);
-    n = n < 0 ? 0 : (int)cap;
+    n = n < 0 ? 0 : a.cap;
   }
   return n;
 }
-__device__ __forceinline__ int seq_tiles(const AttnArgs& a, int b) { return (seq_len(a, b) + kTile - 1) / kTile; }
+__device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
 
-__device__ __forceinline__ int64_t warp_incl_scan(int64_t v) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-    if ((int)(threadIdx.x & 31) >= o) v += u;
+// The list's division (positions fit 31 bits: the host sees to it): the first `big` CTAs take `per`
+// tiles each, the others, which start as those end, `small` tiles. SMs do not run at one speed (the
+// first CTAs of one long sequence ended between 50 and 82 us), so the small runs fill what is left.
+struct Division {
+  int per, small, big;
+  __device__ __forceinline__ Division(const AttnArgs& a, int total) {
+    big = a.big;
+    const int rest = a.ctas - a.big;
+    if (rest == 0) {
+      per = max(a.min_tiles, (int)(((uint32_t)total + a.ctas - 1) / (uint32_t)a.ctas));
+      small = 1;
+    } else {
+      per = max(a.min_tiles, (int)((float)total * a.share) / big + 1);
+      const int left = total - (int)min((int64_t)total, (int64_t)per * big);
+      small = max(a.min_tiles, (int)(((uint32_t)left + rest - 1) / (uint32_t)rest));
+    }
   }
-  return v;
-}
-
-// Tiles of the sequences before `upto`, and of all (warp-collective).
-__device__ __forceinline__ void tiles_before_and_all(const AttnArgs& a, int upto, int64_t& before, int64_t& all) {
-  before = all = 0;
-#pragma unroll 4
-  for (int b = threadIdx.x & 31; b < a.B; b += 32) {
-    const int t = seq_tiles(a, b);
-    all += t;
-    if (b < upto) before += t;
+  __device__ __forceinline__ int64_t begin(int c) const {
+    return c < big ? (int64_t)c * per : (int64_t)big * per + (int64_t)(c - big) * small;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
+  __device__ __forceinline__ int size(int c) const { return c < big ? per : small; }
+  __device__ __forceinline__ int cta_of(int pos) const {
+    const int64_t edge = (int64_t)big * per;
+    return pos < edge ? (int)((uint32_t)pos / (uint32_t)per) : big + (int)((uint32_t)(pos - edge) / (uint32_t)small);
   }
-}
+};
 
-__device__ __forceinline__ int64_t tiles_per_cta(const AttnArgs& a, int64_t all) {
-  const int64_t total = all * a.units;
-  // (a 64-bit division costs ten times the 32-bit one)
-  const int64_t even = total < INT_MAX - a.ctas ? (int)((uint32_t)(total + a.ctas - 1) / (uint32_t)a.ctas)
-                                                : (total + a.ctas - 1) / a.ctas;
-  return max((int64_t)a.min_tiles, even);
-}
-
-// All tiles, and the sequence that holds list position cta * per with the tiles before it (b = B
-// where the list has no such position). Warp-collective; the lengths of up to 128 sequences are read
-// once, of more twice.
-__device__ __forceinline__ void find_start(const AttnArgs& a, int64_t cta, int64_t& total, int64_t& per, int& b,
-                                           int64_t& before) {
+// Where a CTA's run begins: the sequence that holds its first position, that sequence's length and the
+// tiles before it; false where the list ends before. Warp-collective; the lengths of up to 128
+// sequences are read once, of more twice.
+struct Start { int pos, size, total, b, len, before; };
+__device__ __forceinline__ bool find_start(const AttnArgs& a, int cta, Start& st) {
   constexpr int kHeld = 4;
   const int lane = threadIdx.x & 31;
   int held[kHeld];
-  int64_t all = 0;
+  uint32_t all = 0;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < a.B ? seq_tiles(a, 32 * i + lane) : 0;
+  for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < a.B ? seq_len(a, 32 * i + lane) : 0;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) all += held[i];
-  for (int s = 32 * kHeld + lane; s < a.B; s += 32) all += seq_tiles(a, s);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-  total = all * a.units;
-  per = tiles_per_cta(a, all);
-  const int64_t pos = cta * per;
-  b = a.B;
-  before = 0;
-  if (pos >= total) return;
-  int64_t done = 0;
+  for (int i = 0; i < kHeld; ++i) all += tiles_of(held[i]);
+  for (int s = 32 * kHeld + lane; s < a.B; s += 32) all += tiles_of(seq_len(a, s));
+  st.total = (int)__reduce_add_sync(0xffffffffu, all) * a.units;
+  const Division div(a, st.total);
+  const int64_t pos = div.begin(cta);
+  if (pos >= st.total) return false;
+  st.pos = (int)pos;
+  st.size = min(div.size(cta), st.total - st.pos);
+  int done = 0;
+#pragma unroll 1
   for (int base = 0; base < a.B; base += 32) {
-    int mine = 0;
+    int len = 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) mine = base == 32 * i ? held[i] : mine;
-    if (base >= 32 * kHeld) mine = base + lane < a.B ? seq_tiles(a, base + lane) : 0;
-    const int64_t incl = done + warp_incl_scan(mine);
-    const uint32_t hit = __ballot_sync(0xffffffffu, pos < incl * a.units);
+    for (int i = 0; i < kHeld; ++i) len = base == 32 * i ? held[i] : len;
+    if (base >= 32 * kHeld) len = base + lane < a.B ? seq_len(a, base + lane) : 0;
+    const int mine = tiles_of(len);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    incl += done;
+    const uint32_t hit = __ballot_sync(0xffffffffu, st.pos < incl * a.units);
     if (hit) {
       const int s = __ffs(hit) - 1;
-      b = base + s;
-      before = __shfl_sync(0xffffffffu, incl - mine, s);
-      return;
+      st.b = base + s;
+      st.len = __shfl_sync(0xffffffffu, len, s);
+      st.before = __shfl_sync(0xffffffffu, incl - mine, s);
+      return true;
     }
     done = __shfl_sync(0xffffffffu, incl, 31);
   }
+  return false;
 }
 
 // A CTA's run of the list, one (sequence, unit) at a time: the fields describe the current part.
@@ -296,14 +301,14 @@ struct Parts {
   int tile0, tile1, len;
   int slot;                // workspace slot, or -1: the CTA covers all of the unit and finishes its rows
   int unit, tiles;
-  int64_t left;            // tiles of the run behind this part
+  int left;                // tiles of the run behind this part
 
   __device__ __forceinline__ void set(const AttnArgs& a, int tile, int free_slot) {
     kvh = unit / a.subs;
     const int sub = unit - kvh * a.subs;
     row0 = kvh * a.G + sub * a.rows;
     rows = min(a.rows, a.G - sub * a.rows);
-    const int n = (int)min((int64_t)(tiles - tile), left);
+    const int n = min(tiles - tile, left);
     tile0 = tile;
     tile1 = tile + n;
     left -= n;
@@ -315,21 +320,20 @@ struct Parts {
       b = blockIdx.x / a.units;
       unit = blockIdx.x - b * a.units;
       len = seq_len(a, b);
-      tiles = (len + kTile - 1) / kTile;
+      tiles = tiles_of(len);
       left = tiles;
       set(a, 0, -1);
       return len > 0;
     }
-    int64_t total, per, before;
-    find_start(a, blockIdx.x, total, per, b, before);
-    if (b == a.B) return false;
-    const int64_t pos = (int64_t)blockIdx.x * per;
-    left = min(per, total - pos);
-    len = seq_len(a, b);
-    tiles = (len + kTile - 1) / kTile;
-    const int64_t off = pos - before * a.units;
-    unit = off <= INT_MAX ? (int)((uint32_t)off / (uint32_t)tiles) : (int)(off / tiles);
-    set(a, (int)(off - (int64_t)unit * tiles), 2 * blockIdx.x);
+    Start st;
+    if (!find_start(a, blockIdx.x, st)) return false;
+    left = st.size;
+    b = st.b;
+    len = st.len;
+    tiles = tiles_of(len);
+    const int off = st.pos - st.before * a.units;
+    unit = (int)((uint32_t)off / (uint32_t)tiles);
+    set(a, off - unit * tiles, 2 * blockIdx.x);
     return true;
   }
   __device__ __forceinline__ bool next(const AttnArgs& a) {
@@ -340,7 +344,7 @@ struct Parts {
         ++b;
         len = seq_len(a, b);
       } while (len == 0);
-      tiles = (len + kTile - 1) / kTile;
+      tiles = tiles_of(len);
     }
     set(a, 0, 2 * blockIdx.x + 1);
     return true;
@@ -581,7 +585,7 @@ template <int D> struct Tile {
   }
 };
 // Tiles in each warp's ring.
-template <int D> constexpr int ring_stages() { return D <= 64 ? 4 : 2; }
+template <int D> constexpr int ring_stages() { return D <= 64 ? 3 : 2; }
 template <int D> constexpr int attn_smem() {
   return kAttnWarps * (ring_stages<D>() * Tile<D>::kStage + 4 * (D + 4) * 4) + 256;
 }
@@ -592,12 +596,13 @@ template <typename T, int D, bool PAGE16>
 struct TileFetch {
   using L = Tile<D>;
   static constexpr int S = ring_stages<D>();
+  static constexpr bool kWholeRows = D != 96;  // a copy takes whole rows: pointers advance by equal steps
   const AttnArgs& a;
   const int lane, warp;
   Parts p;
   bool more;        // p is a part with tiles left to fetch
   int next;         // next tile of it
-  const T *kb, *vb; // the part's key head in page 0
+  const T *kb, *vb; // the part's key head in page 0 (whole-row copies: this lane's piece of its first row)
   // where the tiles are: PAGE16: lane i has (page, slot) of tile first + 4 i, `have` of them left; else
   // lane i < 16 of token i of the next tile. page -1: not to be read.
   int pg, sl, have;
@@ -616,6 +621,10 @@ struct TileFetch {
     have = 0;
     kb = (const T*)a.k_cache + p.kvh * a.kc_sh;
     vb = (const T*)a.v_cache + p.kvh * a.vc_sh;
+    if constexpr (kWholeRows) {
+      kb += lane / L::kPieces * a.kc_ss + lane % L::kPieces * 8;
+      vb += lane / L::kPieces * a.vc_ss + lane % L::kPieces * 8;
+    }
   }
 
   __device__ __forceinline__ void lookup(int tok, bool on) {
@@ -655,11 +664,9 @@ struct TileFetch {
       if (PAGE16 && mask == 0xFFFFu) {
         const T* kp = kb + (int64_t)page * a.kc_sp + (int64_t)slot * a.kc_ss;
         const T* vp = vb + (int64_t)page * a.vc_sp + (int64_t)slot * a.vc_ss;
-        if constexpr (D != 96) {  // whole rows a copy: pointers advance by the same step
+        if constexpr (kWholeRows) {
           constexpr int kRows = 32 / L::kPieces;
           const int t0 = lane / L::kPieces, piece = lane % L::kPieces;
-          kp += t0 * a.kc_ss + piece * 8;
-          vp += t0 * a.vc_ss + piece * 8;
 #pragma unroll
           for (int i = 0; i < L::kCopies; ++i) {
             cp16(stage + L::k_at(i * kRows + t0, piece), kp);
@@ -679,14 +686,17 @@ struct TileFetch {
           }
         }
       } else {
+        // (from the head's first value again)
+        const T* k0 = (const T*)a.k_cache + p.kvh * a.kc_sh;
+        const T* v0 = (const T*)a.v_cache + p.kvh * a.vc_sh;
 #pragma unroll
         for (int i = 0; i < L::kCopies; ++i) {
           const int u = i * 32 + lane, t = u / L::kPieces, piece = u - t * L::kPieces;
           const int tp = PAGE16 ? page : __shfl_sync(0xffffffffu, pg, t);
           const int64_t ts = PAGE16 ? slot + t : __shfl_sync(0xffffffffu, sl, t);
           const bool on = mask >> t & 1;
-          cp16_if(stage + L::k_at(t, piece), on ? kb + tp * a.kc_sp + ts * a.kc_ss + piece * 8 : kb, on);
-          cp16_if(stage + L::v_at(t, piece), on ? vb + tp * a.vc_sp + ts * a.vc_ss + piece * 8 : vb, on);
+          cp16_if(stage + L::k_at(t, piece), on ? k0 + tp * a.kc_sp + ts * a.kc_ss + piece * 8 : k0, on);
+          cp16_if(stage + L::v_at(t, piece), on ? v0 + tp * a.vc_sp + ts * a.vc_ss + piece * 8 : v0, on);
         }
       }
       next += kAttnWarps;
@@ -701,7 +711,7 @@ struct TileFetch {
 };
 
 template <typename T, int D, int NG, bool PAGE16>
-__global__ void __launch_bounds__(32 * kAttnWarps, NG == 1 ? 3 : 2) attn_mma_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(32 * kAttnWarps, attn_ctas(D, NG)) attn_mma_kernel(const AttnArgs a) {
   using W = TileFetch<T, D, PAGE16>;
   using L = Tile<D>;
   constexpr int KC = D / 32, MT = D / 16;
@@ -740,9 +750,11 @@ __global__ void __launch_bounds__(32 * kAttnWarps, NG == 1 ? 3 : 2) attn_mma_ker
       }
     float o[NG][MT][4];            // values 16 t + r (+ 8) of heads 2j, 2j + 1
     float m[NG][2], l[NG][2];      // of heads 2j, 2j + 1; the sum over this lane's tokens only
+    float base[NG][2];             // m, or 0 while it is -inf
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       m[g][0] = m[g][1] = -INFINITY;
+      base[g][0] = base[g][1] = 0.f;
       l[g][0] = l[g][1] = 0.f;
 #pragma unroll
       for (int t = 0; t < MT; ++t) o[g][t][0] = o[g][t][1] = o[g][t][2] = o[g][t][3] = 0.f;
@@ -784,6 +796,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, NG == 1 ? 3 : 2) attn_mma_ker
             for (int x = 4; x < 32; x <<= 1) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], x));
             const float mn = fmaxf(m[g][n], mx[n]), alpha = ex2(m[g][n] - max_or_zero(mn));
             m[g][n] = mn;
+            base[g][n] = max_or_zero(mn);
             l[g][n] *= alpha;
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
@@ -794,7 +807,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, NG == 1 ? 3 : 2) attn_mma_ker
         }
         float e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = ex2(z[i] - max_or_zero(m[g][i & 1]));
+        for (int i = 0; i < 4; ++i) e[i] = ex2(z[i] - base[g][i & 1]);
         l[g][0] += e[0] + e[2];
         l[g][1] += e[1] + e[3];
 #pragma unroll
@@ -878,87 +891,107 @@ __global__ void __launch_bounds__(32 * kAttnWarps, NG == 1 ? 3 : 2) attn_mma_ker
   zero_empty<T>(a);
 }
 
-// Combines the parts of each (sequence, query head) that several CTAs share, in list order. One
-// block per sequence and query head: the weights of up to 128 parts are made at once, then threads
-// add the parts' rows, VEC values each, in as many interleaved sums as the block has room for.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
-  __shared__ float s_w[128];
-  __shared__ float s_red[2][4];
-  __shared__ alignas(16) float s_acc[128 * VEC];
+// Combines the parts of each (sequence, query head) that several CTAs share, in list order. One block
+// of NT threads per sequence and query head; threads take the parts' rows, VEC values each, in as many
+// interleaved sums as the block has room for. Each thread's first rows are on their way before the
+// weights of the parts (up to NT at once) are known.
+template <typename T, int VEC, int NT>
+__global__ void __launch_bounds__(NT) attn_join_kernel(const AttnArgs a) {
+  constexpr int kAhead = 4, kWarps = NT / 32;
+  __shared__ float s_w[NT];
+  __shared__ float s_red[2][kWarps];
+  __shared__ alignas(16) float s_acc[NT * VEC];
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq;
-  const int tiles = seq_tiles(a, b);
   const int kvh = h / a.G, sub = (h - kvh * a.G) / a.rows, g = h - kvh * a.G - sub * a.rows;
-  int64_t before, all;
-  tiles_before_and_all(a, b, before, all);
-  const int64_t per = tiles_per_cta(a, all);
-  const int64_t s0 = before * a.units + (int64_t)(kvh * a.subs + sub) * tiles, s1 = s0 + tiles;
-  const int c0 = (int)(s0 / per), c1 = (int)((s1 - 1) / per);
+  const int tiles = tiles_of(seq_len(a, b));
+  uint32_t sum_before = 0, sum_all = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < a.B; i += 32) {
+    const int t = tiles_of(seq_len(a, i));
+    sum_all += t;
+    sum_before += i < b ? t : 0;
+  }
+  const int total = (int)__reduce_add_sync(0xffffffffu, sum_all) * a.units;
+  const Division div(a, total);
+  const int s0 = (int)__reduce_add_sync(0xffffffffu, sum_before) * a.units + (kvh * a.subs + sub) * tiles, s1 = s0 + tiles;
+  const int c0 = tiles ? div.cta_of(s0) : 0, c1 = tiles ? div.cta_of(s1 - 1) : 0;
   // launched while the main kernel still runs; its parts are complete behind this point
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tiles == 0 || c0 == c1) return;  // empty, or finished by the one CTA that had it
+  if (c0 == c1) return;  // empty, or finished by the one CTA that had it
   // the first CTA has the rows in its last slot unless its run starts there
-  const int first = 2 * c0 + (c0 * per < s0 ? 1 : 0);
+  const int first = 2 * c0 + (div.begin(c0) < s0 ? 1 : 0);
   auto row_of = [&](int i) { return (int64_t)(i == 0 ? first : 2 * (c0 + i)) * a.rows + g; };
   const int n = c1 - c0 + 1;
   const int lanes = (a.D + VEC - 1) / VEC, warp = threadIdx.x >> 5;
-  const int nway = lanes >= 128 ? 1 : 128 / lanes;
+  const int nway = lanes >= NT ? 1 : NT / lanes;
   const int way = threadIdx.x / lanes, d = (threadIdx.x - way * lanes) * VEC;
   const bool on = way < nway;
-  float m = -INFINITY, sum = 0.f, acc[2][VEC];  // a block of 128 threads holds up to 256 values in two rounds
+  float m = -INFINITY, sum = 0.f, acc[VEC], more = 0.f;  // more: VEC = 1 and a head wider than the block
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 128) {
-    const int k = min(128, n - i0);
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  auto add = [&](const float (&x)[VEC], float f) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] += x[e] * f;
+  };
+  auto get = [&](int i, float (&x)[VEC]) {
+    const float* src = a.ws_o + row_of(i) * a.D + d;
+    if constexpr (VEC == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+    else x[0] = *src;
+  };
+  for (int i0 = 0; i0 < n; i0 += NT) {
+    const int k = min(NT, n - i0);
+    float x[kAhead][VEC];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (on && way + u * nway < k) get(i0 + way + u * nway, x[u]);
     const int64_t r = row_of(i0 + min((int)threadIdx.x, k - 1));
-    const float pm = (int)threadIdx.x < k ? a.ws_ml[2 * r] : -INFINITY;
-    const float pl = (int)threadIdx.x < k ? a.ws_ml[2 * r + 1] : 0.f;
+    const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + 2 * r);
+    const float pm = (int)threadIdx.x < k ? ml.x : -INFINITY, pl = (int)threadIdx.x < k ? ml.y : 0.f;
     const float wm = warp_max(pm);
     if ((threadIdx.x & 31) == 0) s_red[0][warp] = wm;
     __syncthreads();
-    const float mn = fmaxf(m, fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3])));
-    const float alpha = exp2f(m - max_or_zero(mn));
-    const float w = exp2f(pm - max_or_zero(mn));
+    float mn = m;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, s_red[0][w]);
+    const float alpha = exp2f(m - max_or_zero(mn)), w = exp2f(pm - max_or_zero(mn));
     m = mn;
     s_w[threadIdx.x] = w;
-    const float ws = warp_sum(pl * w);
-    if ((threadIdx.x & 31) == 0) s_red[1][warp] = ws;
+    const float wl = warp_sum(pl * w);
+    if ((threadIdx.x & 31) == 0) s_red[1][warp] = wl;
     __syncthreads();
-    sum = sum * alpha + ((s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]));
+    sum *= alpha;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      acc[0][e] *= alpha;
-      acc[1][e] *= alpha;
-    }
+    for (int y = 0; y < kWarps; ++y) sum += s_red[1][y];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] *= alpha;
+    more *= alpha;
     if (on) {
-#pragma unroll 8
-      for (int i = way; i < k; i += nway) {
-        const float f = s_w[i];
-        const float* src = a.ws_o + row_of(i0 + i) * a.D + d;
-        if constexpr (VEC == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src);
-          acc[0][0] += x.x * f; acc[0][1] += x.y * f; acc[0][2] += x.z * f; acc[0][3] += x.w * f;
-        } else {
-          acc[0][0] += src[0] * f;
-          if (d + 128 < a.D) acc[1][0] += src[128] * f;
-        }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (way + u * nway < k) add(x[u], s_w[way + u * nway]);
+#pragma unroll 4
+      for (int i = way + kAhead * nway; i < k; i += nway) {
+        get(i0 + i, x[0]);
+        add(x[0], s_w[i]);
       }
+      if (VEC == 1 && d + NT < a.D)
+        for (int i = 0; i < k; ++i) more += a.ws_o[row_of(i0 + i) * a.D + d + NT] * s_w[i];
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) s_acc[threadIdx.x * VEC + e] = acc[0][e];
+  for (int e = 0; e < VEC; ++e) s_acc[threadIdx.x * VEC + e] = acc[e];
   __syncthreads();
   if (way != 0 || d >= a.D) return;
   T* out = (T*)a.out + b * a.o_sb + h * a.o_sh;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    float x = acc[0][e];
-    for (int y = 1; y < nway; ++y) x += s_acc[(y * lanes) * VEC + d + e];
-    out[d + e] = from_f32<T>(x * inv);
+    float y = acc[e];
+    for (int w = 1; w < nway; ++w) y += s_acc[w * lanes * VEC + d + e];
+    out[d + e] = from_f32<T>(y * inv);
   }
-  if (VEC == 1 && d + 128 < a.D) out[d + 128] = from_f32<T>(acc[1][0] * inv);
+  if (VEC == 1 && d + NT < a.D) out[d + NT] = from_f32<T>(more * inv);
 }
 
 }  // namespace nfb
@@ -1013,6 +1046,20 @@ int launch_mma(const AttnArgs& a, cudaStream_t st) {
   return p16 ? launch_mma_one<T, D, 2, true>(a, st) : launch_mma_one<T, D, 2, false>(a, st);
 }
 
+template <typename T, int VEC, int NT>
+int launch_join(const AttnArgs& a, cudaStream_t st) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hq));
+  cfg.blockDim = dim3(NT);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, attn_join_kernel<T, VEC, NT>, a);
+}
+
 template <typename T>
 int launch_attn(const AttnArgs& a, bool mma, cudaStream_t st) {
   int rc;
@@ -1032,26 +1079,19 @@ int launch_attn(const AttnArgs& a, bool mma, cudaStream_t st) {
     else rc = launch_plain<T, 8>(a, st);
   }
   if (rc != 0 || a.whole || a.ctas == 1) return rc;  // nothing to join
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.B * a.Hq));
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  const bool vec = a.D % 4 == 0 && aligned16(a.ws_o);
-  return (int)(vec ? cudaLaunchKernelEx(&cfg, attn_join_kernel<T, 4>, a) : cudaLaunchKernelEx(&cfg, attn_join_kernel<T, 1>, a));
+  // (the second threshold: one long sequence has tens of parts a head)
+  const bool vec = a.D % 4 == 0 && aligned16(a.ws_o), wide = a.ctas >= 16 * a.B * a.units;
+  if (vec) return wide ? launch_join<T, 4, 512>(a, st) : launch_join<T, 4, 128>(a, st);
+  return launch_join<T, 1, 128>(a, st);
 }
 
-// The split of a call into units and CTAs. Short caches (up to 48 tiles a sequence): one CTA for each
-// (sequence, unit), one launch (400 tokens, 8 sequences of 8 key heads of 128: 7.6 us, divided 10 us;
-// 1000 tokens, 4 sequences: 13.1 us, divided 11.5 us). Else the list is divided over as many CTAs as
-// the GPU holds; where there is much work for each of them and many sequences, over twice as many,
-// which evens out SMs of different speed (64 ragged sequences of up to 3392: 78 us against 84; but one
-// of 131001: 90 us against 97, its join grows).
-void plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool mma, int sms, AttnArgs& a) {
+// The split of a call into units and CTAs; false where positions of the list would not fit 31 bits.
+// Short caches (up to 48 tiles a sequence): one CTA for each (sequence, unit), one launch (400 tokens,
+// 8 sequences of 8 key heads of 128: 7.6 us, divided 10 us; 1000 tokens, 4 sequences: 12.4 us, divided
+// 10 us). Else the list is divided over as many CTAs as the GPU holds; where there is much work for
+// each of them, they take 80% of it and as many smaller runs follow (64 ragged sequences of up to 3392:
+// 75 us against 84; all of 3392: 137 us against 140).
+bool plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool mma, int sms, AttnArgs& a) {
   a.B = (int)B;
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
@@ -1065,18 +1105,26 @@ void plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool 
     a.subs = (a.G + a.rows - 1) / a.rows;
   }
   a.units = a.Hkv * a.subs;
-  if (capacity > INT_MAX - 2 * kTile) capacity = INT_MAX - 2 * kTile;
-  const int64_t pairs = B * a.units, per_seq = (capacity + kTile - 1) / kTile;
-  const int64_t slots = (int64_t)sms * (!mma ? 4 : a.rows <= 8 ? 3 : 2);
+  a.cap = (int)(capacity < INT_MAX - 2 * kTile ? capacity : INT_MAX - 2 * kTile);
+  const int64_t pairs = B * a.units, per_seq = (a.cap + kTile - 1) / kTile;
+  const int64_t slots = (int64_t)sms * (mma ? attn_ctas(a.D, a.rows <= 8 ? 1 : 2) : 4);
   a.min_tiles = kAttnWarps;
+  a.share = 0.f;
   a.whole = per_seq <= 48 && pairs <= INT_MAX;
   if (a.whole) {
-    a.ctas = (int)pairs;
-  } else {
-    const int64_t want = (pairs * per_seq + a.min_tiles - 1) / a.min_tiles;
-    const int64_t most = pairs * per_seq >= 96 * slots && 4 * pairs >= slots ? 2 * slots : slots;
-    a.ctas = (int)(want < 1 ? 1 : want < most ? want : most);
+    a.ctas = a.big = (int)pairs;
+    return true;
   }
+  if (per_seq * pairs > INT_MAX) return false;
+  const int64_t want = (pairs * per_seq + a.min_tiles - 1) / a.min_tiles;
+  if (want >= 2 * slots && pairs * per_seq >= 96 * slots) {
+    a.big = (int)slots;
+    a.ctas = (int)(2 * slots);
+    a.share = 0.8f;
+  } else {
+    a.ctas = a.big = (int)(want < 1 ? 1 : want < slots ? want : slots);
+  }
+  return true;
 }
 
 int64_t ws_floats(const AttnArgs& a) { return a.whole ? 0 : (int64_t)2 * a.ctas * a.rows * (a.D + 2); }
@@ -1124,9 +1172,9 @@ NFB_API int nfb_append_kv(int dtype, const void* q, const void* k, const void* v
 
 NFB_API int64_t nfb_paged_attn_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity) {
   AttnArgs a;
-  plan(B, Hq, Hkv, D, capacity, false, nfb_num_sms(), a);
+  if (!plan(B, Hq, Hkv, D, capacity, false, nfb_num_sms(), a)) return -1;
   const int64_t n = ws_floats(a);
-  plan(B, Hq, Hkv, D, capacity, true, nfb_num_sms(), a);
+  if (!plan(B, Hq, Hkv, D, capacity, true, nfb_num_sms(), a)) return -1;
   return n > ws_floats(a) ? n : ws_floats(a);
 }
 
@@ -1147,7 +1195,7 @@ NFB_API int nfb_paged_attn(int dtype, const void* q, const void* k_cache, const 
              (reinterpret_cast<uintptr_t>(out) & 7) == 0;
   const int piece[] = {7, 8, 11, 12, 13, 14, 15, 16};
   for (int i : piece) mma = mma && dims[i] % 8 == 0;
-  plan(B, Hq, Hkv, D, dims[4] * dims[6], mma, nfb_num_sms(), a);
+  if (!plan(B, Hq, Hkv, D, dims[4] * dims[6], mma, nfb_num_sms(), a)) return (int)cudaErrorInvalidValue;
   a.page_size = (int)dims[4]; a.n_pages = (int)dims[5]; a.table_width = (int)dims[6];
   a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.out = out; a.table = table; a.lengths = lengths;
   a.ws_o = ws;
