@@ -226,12 +226,13 @@ def int64s(*values: int):
 
 
 _NO_GUARD = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(device: torch.device):
     """Context in which ``device`` is current (kernels launch on the current device)."""
     idx = device.index
-    if idx is None or idx == torch.cuda.current_device():
+    if idx is None or idx == _current_device():
         return _NO_GUARD
     return torch.cuda.device(idx)
 

@@ -576,7 +576,7 @@ template <int D> struct Tile {
   static constexpr int kPieces = D / 8;                              // 16-byte pieces of a row
   static constexpr int kPitch = D == 32 ? 64 : D == 64 ? 128 : 256;  // D = 96: padded, the permutation needs it
   static constexpr int kV = kTile * kPitch, kStage = 2 * kV;
-  static constexpr int kCopies = kTile * kPieces / 32;               // copies a lane makes for each of K and V
+  static constexpr int kCopies = kTile * kPieces / 32;               // 16-byte copies a lane makes for each of K and V
   static __device__ __forceinline__ int k_at(int t, int piece) {
     return t * kPitch + ((D == 32 ? piece : piece ^ ((t & 1) << 2)) << 4);
   }
@@ -596,13 +596,13 @@ template <typename T, int D, bool PAGE16>
 struct TileFetch {
   using L = Tile<D>;
   static constexpr int S = ring_stages<D>();
-  static constexpr bool kWholeRows = D != 96;  // a copy takes whole rows: pointers advance by equal steps
+  static constexpr int kRows = 32 / L::kPieces;  // whole rows a copy, so that pointers advance by equal steps (D = 96: 24 lanes)
   const AttnArgs& a;
   const int lane, warp;
   Parts p;
   bool more;        // p is a part with tiles left to fetch
   int next;         // next tile of it
-  const T *kb, *vb; // the part's key head in page 0 (whole-row copies: this lane's piece of its first row)
+  const T *kb, *vb; // this lane's piece of the part's key head, in page 0
   // where the tiles are: PAGE16: lane i has (page, slot) of tile first + 4 i, `have` of them left; else
   // lane i < 16 of token i of the next tile. page -1: not to be read.
   int pg, sl, have;
@@ -621,10 +621,8 @@ struct TileFetch {
     have = 0;
     kb = (const T*)a.k_cache + p.kvh * a.kc_sh;
     vb = (const T*)a.v_cache + p.kvh * a.vc_sh;
-    if constexpr (kWholeRows) {
-      kb += lane / L::kPieces * a.kc_ss + lane % L::kPieces * 8;
-      vb += lane / L::kPieces * a.vc_ss + lane % L::kPieces * 8;
-    }
+    kb += lane / L::kPieces * a.kc_ss + lane % L::kPieces * 8;
+    vb += lane / L::kPieces * a.vc_ss + lane % L::kPieces * 8;
   }
 
   __device__ __forceinline__ void lookup(int tok, bool on) {
@@ -664,25 +662,17 @@ struct TileFetch {
       if (PAGE16 && mask == 0xFFFFu) {
         const T* kp = kb + (int64_t)page * a.kc_sp + (int64_t)slot * a.kc_ss;
         const T* vp = vb + (int64_t)page * a.vc_sp + (int64_t)slot * a.vc_ss;
-        if constexpr (kWholeRows) {
-          constexpr int kRows = 32 / L::kPieces;
-          const int t0 = lane / L::kPieces, piece = lane % L::kPieces;
+        const int t0 = lane / L::kPieces, piece = lane % L::kPieces;
+        if (32 % L::kPieces == 0 || t0 < kRows) {
 #pragma unroll
-          for (int i = 0; i < L::kCopies; ++i) {
-            cp16(stage + L::k_at(i * kRows + t0, piece), kp);
+          for (int t = 0; t < kTile; t += kRows) {
+            cp16(stage + L::k_at(t + t0, piece), kp);
             kp += kRows * a.kc_ss;
           }
 #pragma unroll
-          for (int i = 0; i < L::kCopies; ++i) {
-            cp16(stage + L::v_at(i * kRows + t0, piece), vp);
+          for (int t = 0; t < kTile; t += kRows) {
+            cp16(stage + L::v_at(t + t0, piece), vp);
             vp += kRows * a.vc_ss;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < L::kCopies; ++i) {
-            const int u = i * 32 + lane, t = u / L::kPieces, piece = u - t * L::kPieces;
-            cp16(stage + L::k_at(t, piece), kp + t * a.kc_ss + piece * 8);
-            cp16(stage + L::v_at(t, piece), vp + t * a.vc_ss + piece * 8);
           }
         }
       } else {

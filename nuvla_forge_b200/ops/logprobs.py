@@ -71,19 +71,31 @@ class _TokenLogprobs(torch.autograd.Function):
         return logprobs, entropy, top, ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, g_top, _):
+        # (the wrapper for double differentiation only where a graph of the gradient is wanted: it costs
+        # as much host time as the launch)
+        if torch.is_grad_enabled():
+            return _first_order(ctx, g_logprobs, g_entropy, g_top)
+        return _TokenLogprobs._gradient(ctx, g_logprobs, g_entropy, g_top)
+
+    @staticmethod
+    def _gradient(ctx, g_logprobs, g_entropy, g_top):
         x, targets, stats, entropy, ids = ctx.saved_tensors
         if g_logprobs is None and g_entropy is None and g_top is None:
             return None, None, None, None
         M, V = x.shape
         g_logprobs, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logprobs, g_entropy, g_top))
-        dx = torch.empty((M, V), dtype=x.dtype, device=x.device)
-        with nat.on_device(x.device):
+        dev = x.device
+        dx = torch.empty((M, V), dtype=x.dtype, device=dev)
+        with nat.on_device(dev):
             nat.call("nfb_logprobs_bwd", nat.DT[x.dtype], x.data_ptr(), x.stride(0), M, V, nat.ptr(targets),
                      ctx.ignore_index, ctx.top_k, nat.ptr(ids), nat.ptr(g_logprobs), nat.ptr(g_entropy),
-                     nat.ptr(g_top), stats.data_ptr(), entropy.data_ptr(), dx.data_ptr(), nat.stream(x.device))
+                     nat.ptr(g_top), stats.data_ptr(), entropy.data_ptr(), dx.data_ptr(), nat.stream(dev))
         return dx, None, None, None
+
+
+# gradients of the gradient raise instead of being silently zero
+_first_order = once_differentiable(_TokenLogprobs._gradient)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top_k: int = 0,
@@ -95,7 +107,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     ``ignore_index`` has log p 0 and no gradient; its row's entropy and alternatives are computed all the
     same. A masked logit is -inf; a row of nothing else has log p -inf, entropy 0 and no gradient. A row
     with a NaN or +inf logit gives NaN (and unspecified alternatives). A target outside the vocabulary
-    gives NaN and is reported by ``check_status`` (on the CPU it raises).
+    gives NaN and is reported by ``check_status`` (on the CPU it raises). Nothing waits for the host; a call
+    can be captured in a CUDA graph after a first one outside of it.
     """
     if logits.dim() < 1 or not logits.is_floating_point():
         raise TypeError(f"logits must be a floating-point tensor [..., V], got {tuple(logits.shape)} {logits.dtype}")

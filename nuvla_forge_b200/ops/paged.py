@@ -9,7 +9,8 @@ Layout: pools ``[n_pages, page_size, Hkv, D]`` for keys and values (the projecti
 ``ops.attention``), ``page_table`` [B, W] int32 page ids, ``lengths`` [B] int32. Token p of sequence
 b is in page ``page_table[b, p // page_size]``, slot ``p % page_size``; any page size works. Lengths
 and page ids stay on the device: neither op waits for the host, both can be captured in a CUDA
-graph, and several streams can run them at once on caches of their own.
+graph (after a first call outside of one, which creates the device's status word), and several
+streams can run them at once on caches of their own.
 
 A position or page id out of range cannot be refused without reading it back: the kernels skip the
 token and set a status word that ``check_status`` (and the trainer's health monitor) raises on. On
@@ -52,7 +53,7 @@ def _check_cache(k_cache, v_cache, page_table, lengths, like, heads: int, dim: i
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"k_cache and v_cache must both be [n_pages, page_size, Hkv, D], got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    if k_cache.shape[1] < 1 or k_cache.shape[2] != heads or k_cache.shape[3] != dim:
+    if heads < 1 or dim < 1 or k_cache.shape[1] < 1 or k_cache.shape[2] != heads or k_cache.shape[3] != dim:
         raise ValueError(f"cache {tuple(k_cache.shape)} does not hold {heads} heads of {dim}")
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         raise ValueError("the cache's last dimension must be contiguous")
@@ -66,11 +67,6 @@ def _check_cache(k_cache, v_cache, page_table, lengths, like, heads: int, dim: i
     dev = like.device
     if not (k_cache.device == v_cache.device == page_table.device == lengths.device == dev):
         raise ValueError("all tensors must be on one device")
-
-
-def _check_no_grad(op: str, *tensors) -> None:
-    if any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{op} has no backward pass: call it under torch.no_grad()")
 
 
 def _inner(t: torch.Tensor) -> torch.Tensor:
@@ -162,8 +158,9 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if plan is None:
         plan = _append_plan(key, k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
     native, dims = plan
-    if torch.is_grad_enabled():
-        _check_no_grad("append_kv", k, v, q, k_cache, v_cache)
+    if (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+            or (q is not None and q.requires_grad)) and torch.is_grad_enabled():
+        raise RuntimeError("append_kv has no backward pass: call it under torch.no_grad()")
     if force_reference or not native:
         out = append_kv_ref(k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
         return out.clone() if out is q and q is not None else out
@@ -199,6 +196,9 @@ def _attention_plan(key, q, k_cache, v_cache, page_table, lengths) -> tuple:
         dims = nat.int64s(B, Hq, Hkv, D, ps, n_pages, W, q.stride(0), q.stride(2), Hq * D, D, *k_cache.stride()[:3],
                           *v_cache.stride()[:3], page_table.stride(0))
         ws = int(nat.lib().nfb_paged_attn_ws(B, Hq, Hkv, D, ps * W))
+        if ws < 0:
+            raise ValueError(f"{B} sequences of up to {ps * W} tokens and {Hkv} key heads are more than the kernel's "
+                             f"2^31 (sequence, head, 16-token tile) units: narrow the page table")
     return _keep(key, (native, dims, ws, D ** -0.5))
 
 
@@ -216,8 +216,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if plan is None:
         plan = _attention_plan(key, q, k_cache, v_cache, page_table, lengths)
     native, dims, n_ws, default = plan
-    if torch.is_grad_enabled():
-        _check_no_grad("paged_attention", q, k_cache, v_cache)
+    if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("paged_attention has no backward pass: call it under torch.no_grad()")
     sc = default if scale is None else float(scale)
     if force_reference or not native:
         return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, sc)

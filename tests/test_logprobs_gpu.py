@@ -216,6 +216,14 @@ def test_gradient_of_each_output_alone_and_of_an_empty_batch():
     assert leaf.grad.shape == (0, 10)
 
 
+def test_second_derivatives_are_refused():
+    x, t = _logits(3, 100, torch.float32, seed=12)
+    leaf, w = x.requires_grad_(True), torch.ones(3, device=DEV, requires_grad=True)
+    (dx,) = torch.autograd.grad((token_logprobs(leaf, t).logprobs * w).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.square().sum().backward()
+
+
 def test_gradient_against_differences():
     """Directional central differences of the 64-bit function; the gradient is computed in fp32."""
     x, t = _logits(3, 501, torch.float32, seed=6)

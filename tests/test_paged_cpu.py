@@ -70,6 +70,7 @@ def test_append_refusals():
     bad = [
         (ValueError, dict(k=a["k"][0])),
         (ValueError, dict(v=a["v"][:, :2])),
+        (ValueError, dict(k=a["k"][:, :, :0], v=a["v"][:, :, :0], k_cache=a["k_cache"][:, :, :0], v_cache=a["v_cache"][:, :, :0])),
         (ValueError, dict(k_cache=a["k_cache"][..., :4], v_cache=a["v_cache"][..., :4])),
         (ValueError, dict(k_cache=a["k_cache"][0])),
         (ValueError, dict(k_cache=a["k_cache"].transpose(2, 3).contiguous().transpose(2, 3))),
@@ -132,6 +133,8 @@ def test_paged_attention_refusals():
         (ValueError, dict(q=torch.randn(1, 1, 3, 8))),
         (ValueError, dict(q=torch.randn(1, 1, 4, 4))),
         (ValueError, dict(q=torch.randn(2, 1, 4, 8))),
+        (ValueError, dict(q=torch.randn(1, 1, 4, 0), k_cache=kc[..., :0], v_cache=vc[..., :0])),
+        (ValueError, dict(k_cache=kc[:, :, :0], v_cache=vc[:, :, :0])),
         (ValueError, dict(v_cache=vc[:5])),
         (ValueError, dict(k_cache=kc[0])),
         (TypeError, dict(k_cache=kc.half(), v_cache=vc.half())),

@@ -327,6 +327,32 @@ def test_refusals_on_the_gpu():
             paged_attention(**{**dict(q=k, k_cache=kc, v_cache=vc, page_table=table, lengths=n), **bad})
     with pytest.raises(RuntimeError, match="no_grad"):
         paged_attention(k.requires_grad_(True), kc, vc, table, n)
+    wide = table[:, :1].expand(1, 2 ** 27)                   # a table (of one entry) for 2^31 tokens
+    with pytest.raises(ValueError, match="narrow the page table"):
+        paged_attention(torch.zeros(1, 1, 64, 64, device=DEV), torch.zeros(4, 16, 64, 64, device=DEV),
+                        torch.zeros(4, 16, 64, 64, device=DEV), wide, n)
+
+
+def test_mixed_calls_and_other_current_stream():
+    """The same shapes with other strides, types and options use plans of their own."""
+    g = _gen(16)
+    for dtype in (torch.bfloat16, torch.float32, torch.bfloat16):
+        for heads_first in (False, True):
+            for pairs in (False, True):
+                kc, vc = _pool(6, 16, 2, 64, dtype, g)
+                if heads_first:
+                    kc, vc = (c.transpose(1, 2).contiguous().transpose(1, 2) for c in (kc, vc))
+                table = torch.tensor([[3, 1]], dtype=torch.int32, device=DEV)
+                start = torch.tensor([13], dtype=torch.int32, device=DEV)
+                k, v, q = (torch.randn(1, 1, h, 64, generator=g, device=DEV).to(dtype) for h in (2, 2, 4))
+                ang = torch.rand(20, 32, generator=g, device=DEV) * 6
+                rk, rv, rq = _append64(k, v, kc, vc, table, start, None, q, ang.cos(), ang.sin(), pairs)
+                out = append_kv(k, v, kc, vc, table, start, q=q, cos=ang.cos(), sin=ang.sin(), interleaved=pairs)
+                eps = torch.finfo(dtype).eps / 2
+                for x, r in ((kc, rk), (vc, rv), (out, rq)):
+                    assert ((x.double() - r).abs() <= eps * r.abs() + 48 * 2.0 ** -24).all()
+                n = start + 1
+                _check_attention(paged_attention(out, kc, vc, table, n), out, kc, vc, table, n)
 
 
 def test_offsets_past_32_bits():
