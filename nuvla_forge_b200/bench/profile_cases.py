@@ -236,6 +236,59 @@ def attn_fwd(iters):
     flash_attn.check_status()
 
 
+def _paged(batch, length, lengths):
+    """bf16 pools for the 1b backbone's heads (16 queries, 8 keys of 128), pages of 64 tokens, scattered."""
+    per = -(-length // 64)
+    kc, vc = (_bf(batch * per, 64, 8, 128, seed=i) for i in range(2))
+    table = torch.randperm(batch * per, generator=torch.Generator().manual_seed(0)).view(batch, per).to("cuda", torch.int32)
+    return kc, vc, table, torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+
+@case
+def paged_attn(iters):
+    """One query each of 64 sequences over 3392 cached tokens (890 MB of keys and values)."""
+    from ..ops import paged_attention
+    kc, vc, table, n = _paged(64, 3392, [3392] * 64)
+    q = _bf(64, 1, 16, 128, seed=2)
+    for _ in range(iters):
+        paged_attention(q, kc, vc, table, n)
+
+
+@case
+def append_kv(iters):
+    """8 contexts of 3392 tokens rotated and stored (16 query, 8 key heads of 128)."""
+    from ..ops import append_kv as op
+    kc, vc, table, n = _paged(8, 3392, [0] * 8)
+    q, k, v = _bf(8, 3392, 32, 128, seed=2).split([16, 8, 8], dim=2)
+    ang = torch.rand(3392, 64, device="cuda") * 6
+    cos, sin = ang.cos(), ang.sin()
+    for _ in range(iters):
+        op(k, v, kc, vc, table, n, q=q, cos=cos, sin=sin)
+
+
+def _scores(iters, top_k, backward):
+    from ..ops import token_logprobs
+    x = _bf(8192, 32000).requires_grad_(backward)
+    t = torch.randint(0, 32000, (8192,), device="cuda")
+    g = torch.randn(8192, device="cuda")
+    for _ in range(iters):
+        r = token_logprobs(x, t, top_k=top_k)
+        if backward:
+            torch.autograd.grad([r.logprobs, r.entropy], x, [g, g])
+
+
+@case
+def logprobs_fwd(iters):
+    """Log probabilities, entropy and 5 alternatives of 8192 x 32000 bf16 logits (524 MB)."""
+    _scores(iters, 5, False)
+
+
+@case
+def logprobs_bwd(iters):
+    """The gradient of log probabilities and entropy for 8192 x 32000 bf16 logits."""
+    _scores(iters, 0, True)
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--case", required=True, choices=sorted(CASES))

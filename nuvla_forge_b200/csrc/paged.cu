@@ -36,13 +36,27 @@ enum PagedSite : uint32_t { kSiteAppendPos = 1, kSiteAppendPage = 2, kSiteAppend
 // ---------------------------------------------------------------------------------------------
 constexpr int kAppendThreads = 128;
 
+// Division of numbers below 2^31 by a fixed one: n / d = n m >> (31 + s) with s = ceil(log2 d) and
+// m = ceil(2^(31 + s) / d), since then m d - 2^(31 + s) < d <= 2^s and n (m d - 2^(31 + s)) < 2^(31 + s).
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ void set(uint32_t div) {
+    d = div;
+    s = 0;
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int quot(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> (31 + s)); }
+};
+
 struct AppendArgs {
   const void *q, *k, *v;
   void *q_out, *k_cache, *v_cache;
   const int32_t *table, *starts, *counts;
   const float *cos, *sin;
   uint32_t* status;
-  int64_t tokens;  // B * T
+  int token0, tokens;             // the launch's tokens, of B * T
+  FastDiv by_units, by_T, by_rot, by_v, by_page;
   int T, Hq, Hkv, D, half, interleaved, page_size, n_pages, table_width, rope_rows;
   int units, units_rot, units_v;  // of a token; of a head of q or k; of a head of v
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
@@ -102,19 +116,17 @@ __device__ __forceinline__ void turn(Chunk<T, V>& c1, Chunk<T, V>& c2, const flo
 
 template <typename T, int V, bool PAIRS>
 __global__ void __launch_bounds__(kAppendThreads, 12) append_kernel(const AppendArgs a) {
-  const int64_t idx = (int64_t)blockIdx.x * kAppendThreads + threadIdx.x;
-  const int64_t token = idx <= INT_MAX ? (int)((uint32_t)idx / (uint32_t)a.units) : idx / a.units;
-  if (token >= a.tokens) return;
-  int u = (int)(idx - token * a.units);
-  const int b = token <= INT_MAX ? (int)((uint32_t)token / (uint32_t)a.T) : (int)(token / a.T);
-  const int t = (int)(token - (int64_t)b * a.T);
+  const int idx = blockIdx.x * kAppendThreads + threadIdx.x;
+  const int local = a.by_units.quot(idx);
+  if (local >= a.tokens) return;
+  int u = idx - local * a.units;
+  const int token = a.token0 + local, b = a.by_T.quot(token), t = token - b * a.T;
   const bool live = a.counts == nullptr || t < a.counts[b];
   const int q_units = a.Hq * a.units_rot, k_units = a.Hkv * a.units_rot;
   const int kind = u < q_units ? 0 : u < q_units + k_units ? 1 : 2;
   if (kind != 0 && !live) return;
   u -= kind == 0 ? 0 : kind == 1 ? q_units : q_units + k_units;
-  const int per = kind == 2 ? a.units_v : a.units_rot;
-  const int h = u / per, e = u - h * per;
+  const int h = kind == 2 ? a.by_v.quot(u) : a.by_rot.quot(u), e = u - h * (kind == 2 ? a.units_v : a.units_rot);
   // the unit's vectors: a rotated pair of vectors, or up to two neighbours of the rest
   const int n_pair = kind == 2 ? 0 : a.half / V;
   const bool turned = e < n_pair;
@@ -138,14 +150,14 @@ __global__ void __launch_bounds__(kAppendThreads, 12) append_kernel(const Append
   }
   T* dst;
   if (kind == 0) {
-    dst = (T*)a.q_out + (token * a.Hq + h) * a.D;
+    dst = (T*)a.q_out + ((int64_t)token * a.Hq + h) * a.D;
   } else {
     if (!stored) return;
     if (pos < 0 || pos >= (int64_t)a.table_width * a.page_size) {
       set_status(a.status, kBadArgument, kSiteAppendPos);
       return;
     }
-    const int w = pos <= INT_MAX ? (int)((uint32_t)pos / (uint32_t)a.page_size) : (int)(pos / a.page_size);
+    const int w = pos <= INT_MAX ? a.by_page.quot((int)pos) : (int)(pos / a.page_size);
     const int slot = (int)(pos - (int64_t)w * a.page_size);
     const int page = a.table[(int64_t)b * a.t_sb + w];
     if (page < 0 || page >= a.n_pages) {
@@ -998,13 +1010,25 @@ int launch_append(AppendArgs& a, cudaStream_t st) {
   a.units_rot = a.half / V + (rest + 1) / 2;
   a.units_v = (a.D / V + 1) / 2;
   const int64_t units = (int64_t)(a.Hq + a.Hkv) * a.units_rot + (int64_t)a.Hkv * a.units_v;
-  if (units > INT_MAX) return (int)cudaErrorInvalidValue;
+  if (units > INT_MAX / 2) return (int)cudaErrorInvalidValue;
   a.units = (int)units;
-  if (a.tokens > ((int64_t)INT_MAX * kAppendThreads) / units) return (int)cudaErrorInvalidValue;
-  const int64_t blocks = (a.tokens * units + kAppendThreads - 1) / kAppendThreads;
-  if (a.interleaved) append_kernel<T, V, true><<<(unsigned)blocks, kAppendThreads, 0, st>>>(a);
-  else append_kernel<T, V, false><<<(unsigned)blocks, kAppendThreads, 0, st>>>(a);
-  return (int)cudaGetLastError();
+  a.by_units.set((uint32_t)units);
+  a.by_T.set((uint32_t)a.T);
+  a.by_rot.set((uint32_t)a.units_rot);
+  a.by_v.set((uint32_t)a.units_v);
+  a.by_page.set((uint32_t)a.page_size);
+  // thread numbers are kept below 2^31: more tokens take more launches
+  const int all = a.tokens, most = (int)((INT_MAX - kAppendThreads) / units);
+  for (a.token0 = 0; a.token0 < all; a.token0 += a.tokens) {
+    a.tokens = all - a.token0 < most ? all - a.token0 : most;
+    const unsigned blocks = (unsigned)(((int64_t)a.tokens * units + kAppendThreads - 1) / kAppendThreads);
+    if (a.interleaved) append_kernel<T, V, true><<<blocks, kAppendThreads, 0, st>>>(a);
+    else append_kernel<T, V, false><<<blocks, kAppendThreads, 0, st>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    if (a.token0 > INT_MAX - a.tokens) break;
+  }
+  return 0;
 }
 
 template <typename T, int DP>
@@ -1142,7 +1166,8 @@ NFB_API int nfb_append_kv(int dtype, const void* q, const void* k, const void* v
   a.kc_sp = dims[20]; a.kc_ss = dims[21]; a.kc_sh = dims[22];
   a.vc_sp = dims[23]; a.vc_ss = dims[24]; a.vc_sh = dims[25];
   a.t_sb = dims[26];
-  a.tokens = B * a.T;
+  if (B * a.T > INT_MAX) return (int)cudaErrorInvalidValue;
+  a.tokens = (int)(B * a.T);
   if (a.tokens == 0 || a.D == 0 || a.Hkv == 0) return 0;
   if (2 * a.half > a.D || a.page_size < 1 || (a.half > 0 && (a.rope_rows < 1 || !cos || !sin)))
     return (int)cudaErrorInvalidValue;
