@@ -124,22 +124,27 @@ __device__ __forceinline__ float kth_of_warp(float v, int k) {
 //
 // Alternatives: the k-th largest of the maxima of 32 groups of threads bounds the k-th largest logit
 // from below. The bound is taken after every thread's first vectors and renewed as the row goes by (a
-// group maximum that is read late is only a lower bound, so nobody waits); values that reach it are
-// put aside, some k (1 + log(row / first vectors)) of them, and ranked at the end. Where more come
-// (a rising row, a constant or fully masked one) the row is looked at again: with the final bound,
+// group maximum that is read late is only a lower bound, so nobody waits); a thread whose vectors of a
+// round reach it notes their place and maximum, some k (1 + log(rounds)) notes a row. At the end the
+// notes that reach the final bound are read again, from the L2, a warp for each note and a lane for
+// each value, and the candidates (about k) are ranked against one another. (Looking at the values when
+// they come, unrolled over a thread's vectors, filled the loop with code that crowded the instruction
+// cache: 15% of the stalls.) If values equal to the bound overflow (a constant or fully masked row),
 // those above it are ranked and the first ones equal to it taken in the order of the row; if even the
-// greater ones overflow (a sorted row), k rounds of a block-wide maximum remain.
+// greater ones overflow (sorted rows), k rounds of a block-wide maximum remain.
 //
 // What bounds it: 2 bytes a value at the HBM's rate leave 1.4 clocks of an SM quarter's
 // special-function unit for each exponential, which takes 0.25 to 0.5 of that.
-constexpr int kLpUnroll = 4, kLpAbove = 1024, kLpEqual = 256;
+constexpr int kLpUnroll = 4, kLpAbove = 512, kLpEqual = 128;
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a) {
   constexpr int VE = 16 / sizeof(T), kWarps = NT / 32, kGroup = NT / 32;  // 32 groups of kGroup threads
+  constexpr int kNotes = NT == 64 ? 256 : NT == 128 ? 768 : 1024;  // 32 alternatives leave some 130 (1 + log(rounds))
   __shared__ Stat s_stat[kWarps];
   __shared__ float s_group[32];
-  __shared__ int s_above, s_equal;            // values put aside (first look: all of them in s_above)
+  __shared__ int s_noted, s_above, s_equal;   // notes; candidates above the bound and equal to it
+  __shared__ float2 s_note[kNotes];         // a thread's maximum in a round, and the number of its first vector
   __shared__ uint64_t s_cand[kLpAbove + kLpEqual];
   __shared__ uint64_t s_best[kMaxTop];        // keys of the alternatives, descending; 0: none
   __shared__ uint64_t s_round[kWarps];
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
   const int single = tid < n_front ? lo + tid : tid - n_front < n_back ? head + last * VE + (tid - n_front) : -1;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   if (tid < kMaxTop) s_best[tid] = 0;
-  if (tid == 0) s_above = s_equal = 0;
+  if (tid == 0) s_noted = s_above = s_equal = 0;
 
   float mx = single >= 0 ? to_f32(x[single]) : -INFINITY;
   Stat st{-INFINITY, 0.f, 0.f};
@@ -173,6 +178,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
       st.u = st.s * d;
     }
   }
+  const int rounds = (last - first + NT * kLpUnroll - 1) / (NT * kLpUnroll);
   float bound = INFINITY;
   volatile float* group = s_group;
   auto publish = [&](float m) {  // this thread's group maximum so far
@@ -180,49 +186,37 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     for (int o = kGroup / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane % kGroup == 0) group[tid / kGroup] = m;
   };
-  auto aside = [&](float z, int j) {
-    if (z >= bound) {
-      const int at = atomicAdd(&s_above, 1);
-      if (at < kLpAbove) s_cand[at] = rank_key(z, j);
-    }
-  };
-  int turn = 0;
-  for (int base = first; base == first || base < last; base += NT * kLpUnroll, ++turn) {
-    const int v0 = base + tid;
+#pragma unroll 1
+  for (int turn = 0; turn < rounds; ++turn) {
+    const int base = first + turn * (NT * kLpUnroll), v0 = base + tid;
     uint4 w[kLpUnroll];
+    if (base + NT * kLpUnroll <= last) {
 #pragma unroll
-    for (int i = 0; i < kLpUnroll; ++i) {
-      const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
-      w[i] = make_uint4(none, none, none, none);  // -inf
-      if (v0 + i * NT < last) w[i] = ld_row(xv + v0 + i * NT);
-    }
-    float vm[kLpUnroll], m = -INFINITY;
+      for (int i = 0; i < kLpUnroll; ++i) w[i] = ld_row(xv + v0 + i * NT);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kLpUnroll; ++i) {
-      vm[i] = vec_max<T>(w[i]);
-      m = fmaxf(m, vm[i]);
+      for (int i = 0; i < kLpUnroll; ++i) {
+        const uint32_t none = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+        w[i] = make_uint4(none, none, none, none);  // -inf
+        if (v0 + i * NT < last) w[i] = ld_row(xv + v0 + i * NT);
+      }
     }
+    float m = vec_max<T>(w[0]);
+#pragma unroll
+    for (int i = 1; i < kLpUnroll; ++i) m = fmaxf(m, vec_max<T>(w[i]));
     if (m > mx) {
       mx = m;
       st = stat_at(st, mx);
     }
     if (k > 0) {
-      if ((turn & (turn - 1)) == 0) {  // the first vectors, and at 1, 2, 4, ... times as many
+      if ((turn & (turn - 1)) == 0) {  // rounds 0, 1, 2, 4, 8, ...
         publish(mx);
         if (turn == 0) __syncthreads();
         bound = kth_of_warp(group[lane], k);
-        if (turn == 0 && single >= 0) aside(to_f32(x[single]), single);
       }
       if (m >= bound) {
-#pragma unroll
-        for (int i = 0; i < kLpUnroll; ++i) {
-          if (vm[i] >= bound && v0 + i * NT < last) {
-            float z[VE];
-            unpack16<T>(w[i], z);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) aside(z[e], head + (v0 + i * NT) * VE + e);
-          }
-        }
+        const int at = atomicAdd(&s_noted, 1);
+        if (at < kNotes) s_note[at] = make_float2(m, __int_as_float(v0));
       }
     }
     const float ref = or_zero(mx);
@@ -257,52 +251,48 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     t.u = warp_sum(t.u);
     if (lane == 0) s_row = t;
   }
-  const int put = k > 0 ? s_above : 0;
   auto rank_in = [&](const uint64_t* list, int n, uint64_t mine) {
     int better = 0;
     for (int o = 0; o < n; ++o) better += list[o] > mine;
     if (better < k) s_best[better] = mine;
   };
-  if (put <= 192) {
-    for (int i = tid; i < put; i += NT) rank_in(s_cand, put, s_cand[i]);
-  } else if (put <= kLpAbove) {
-    // many: those that the final bound leaves first, since ranking costs the square
+  if (k > 0) {
     bound = kth_of_warp(group[lane], k);
-    uint64_t mine[kLpAbove / NT];
+    auto take = [&](float z, int j) {
+      if (z > bound) {
+        const int at = atomicAdd(&s_above, 1);
+        if (at < kLpAbove) s_cand[at] = rank_key(z, j);
+      } else if (z == bound) {
+        const int at = atomicAdd(&s_equal, 1);
+        if (at < kLpEqual) s_cand[kLpAbove + at] = rank_key(z, j);
+      }
+    };
+    if (single >= 0) take(to_f32(x[single]), single);
+    // lane l of a warp has value l of the vectors from number v0 on, NT apart
+    const int lane_v = lane / VE * NT, lane_e = lane % VE;
+    const bool lane_on = lane < kLpUnroll * VE;
+    const int notes = s_noted;
+    if (notes <= kNotes) {
+      for (int i0 = warp; i0 < notes; i0 += 4 * kWarps) {
+        int j[4];
+        float z[4];
 #pragma unroll
-    for (int i = 0; i < kLpAbove / NT; ++i) mine[i] = tid + i * NT < put ? s_cand[tid + i * NT] : 0;
-    __syncthreads();
-    const uint64_t least = rank_key(bound, -1);  // behind every index: below all keys of its value
-#pragma unroll
-    for (int i = 0; i < kLpAbove / NT; ++i)
-      if (mine[i] >= least) s_cand[atomicAdd(&s_equal, 1)] = mine[i];
-    __syncthreads();
-    const int left = s_equal;
-    for (int i = tid; i < left; i += NT) rank_in(s_cand, left, s_cand[i]);
-  } else {
-    bound = kth_of_warp(group[lane], k);
-    __syncthreads();
-    if (tid == 0) s_above = s_equal = 0;
-    __syncthreads();
-    if (mx >= bound) {
-      auto take = [&](float z, int j) {
-        if (z > bound) {
-          const int at = atomicAdd(&s_above, 1);
-          if (at < kLpAbove) s_cand[at] = rank_key(z, j);
-        } else if (z == bound) {
-          const int at = atomicAdd(&s_equal, 1);
-          if (at < kLpEqual) s_cand[kLpAbove + at] = rank_key(z, j);
+        for (int i = 0; i < 4; ++i) {
+          const float2 n = i0 + i * kWarps < notes ? s_note[i0 + i * kWarps] : make_float2(-INFINITY, 0.f);
+          const int v = __float_as_int(n.y) + lane_v;
+          j[i] = i0 + i * kWarps < notes && n.x >= bound && lane_on && v < last ? head + v * VE + lane_e : -1;
+          if (j[i] >= 0) z[i] = to_f32(x[j[i]]);
         }
-      };
-      if (single >= 0) take(to_f32(x[single]), single);
-#pragma unroll 4
-      for (int v = first + tid; v < last; v += NT) {
-        const uint4 w = __ldg(xv + v);
-        if (vec_max<T>(w) >= bound) {
-          float z[VE];
-          unpack16<T>(w, z);
 #pragma unroll
-          for (int e = 0; e < VE; ++e) take(z[e], head + v * VE + e);
+        for (int i = 0; i < 4; ++i)
+          if (j[i] >= 0) take(z[i], j[i]);
+      }
+    } else {  // too many: every round of the lanes that reach the bound
+      for (uint32_t who = __ballot_sync(0xffffffffu, mx >= bound); who; who &= who - 1) {
+        for (int turn = 0; turn < rounds; ++turn) {
+          const int v = first + turn * (NT * kLpUnroll) + (tid - lane + __ffs(who) - 1) + lane_v;
+          const int j = head + v * VE + lane_e;
+          if (lane_on && v < last) take(to_f32(x[j]), j);
         }
       }
     }
