@@ -133,8 +133,9 @@ __device__ __forceinline__ float kth_of_warp(float v, int k) {
 // those above it are ranked and the first ones equal to it taken in the order of the row; if even the
 // greater ones overflow (sorted rows), k rounds of a block-wide maximum remain.
 //
-// What bounds it: 2 bytes a value at the HBM's rate leave 1.4 clocks of an SM quarter's
-// special-function unit for each exponential, which takes 0.25 to 0.5 of that.
+// What bounds it: for 16-bit logits the HBM's rate leaves 11 issue slots of an SM for a warp's 32 values,
+// and the sums take 8 with one exponential among them. Without alternatives 16384 x 32000 bf16 take
+// 173 us (6.05 TB/s, 94% of the measured copy rate); with 5 the issue slots bind (84% busy): 224 us.
 constexpr int kLpUnroll = 4, kLpAbove = 512, kLpEqual = 128;
 
 template <typename T, int NT>
@@ -209,7 +210,8 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
       st = stat_at(st, mx);
     }
     if (k > 0) {
-      if ((turn & (turn - 1)) == 0) {  // rounds 0, 1, 2, 4, 8, ...
+      // rounds 0, 2, 8, 32, ..., or with many alternatives 0, 1, 2, 4, ... (1500 x 150001 with 32: 206 us, 286 us)
+      if ((turn & (turn - 1)) == 0 && (turn == 0 || k > 8 || (turn & 0x2AAAAAAA))) {
         publish(mx);
         if (turn == 0) __syncthreads();
         bound = kth_of_warp(group[lane], k);
@@ -417,7 +419,8 @@ struct LpBwdArgs {
   int V, top_k, chunks, per;  // CTAs a row; values of a chunk
 };
 
-// Backward: a stream over the row, bound by its bytes (each logit read, each gradient written). With
+// Backward: a stream over the row, bound by its bytes (each logit read, each gradient written: 16384 x
+// 32000 bf16 in 325 us, the measured copy rate). With
 // d = z - m the gradient apart from the given tokens is exp(d) (c1 d + c0), c0 and c1 of the row. The
 // given tokens' places are written again by the first threads, each with its whole value (a token may
 // be the target and an alternative), rounded once.
@@ -508,7 +511,8 @@ namespace {
 
 template <typename T, int NT>
 int launch_fwd_nt(LpArgs& a, cudaStream_t st) {
-  // a cluster for each row while the rows leave SMs idle and each CTA keeps two vectors a thread
+  // a cluster for each row while the rows leave SMs idle and each CTA keeps two vectors a thread (one row
+  // of 150000 fp32 logits 10.8 us, undivided 22.4 us; of 32000 bf16 6.6 us against 7.4 us)
   const int64_t vecs = a.V / (int64_t)(16 / sizeof(T));
   a.split = 1;
   while (a.split < 8 && a.rows * a.split * 2 <= 2 * nfb_num_sms() && vecs >= (int64_t)a.split * 4 * NT) a.split *= 2;
@@ -527,13 +531,14 @@ int launch_fwd_nt(LpArgs& a, cudaStream_t st) {
 }
 
 // Threads a row: few for short rows and where many rows fill the GPU anyway (less waiting for one
-// another: 16384 x 32000 bf16 with 5 alternatives 234 us with 128, 257 us with 256; 20000 x 2000 fp16
-// 48 us with 64, 66 us with 128), many for few rows (64 x 32000 bf16: 7.4 us with 256, 8.7 us with 128).
+// another: 16384 x 32000 bf16 with 5 alternatives 224 us with 128, 274 us with 256; 20000 x 2000 fp16
+// 52 us with 64, 83 us with 128), many for few rows or long ones (64 x 32000 bf16: 7.6 us with 256, 8.2 us
+// with 128; 1500 x 150001 with 32 alternatives 213 us against 458 us).
 template <typename T>
 int launch_fwd(LpArgs& a, cudaStream_t st) {
   const int64_t bytes = a.V * (int64_t)sizeof(T);
   if (bytes < 8192) return launch_fwd_nt<T, 64>(a, st);
-  if (bytes < 16384 || a.rows >= 12 * (int64_t)nfb_num_sms()) return launch_fwd_nt<T, 128>(a, st);
+  if (bytes < 16384 || (bytes <= 131072 && a.rows >= 12 * (int64_t)nfb_num_sms())) return launch_fwd_nt<T, 128>(a, st);
   return launch_fwd_nt<T, 256>(a, st);
 }
 

@@ -29,10 +29,10 @@ enum PagedSite : uint32_t { kSiteAppendPos = 1, kSiteAppendPage = 2, kSiteAppend
 // The call is bound by its bytes (each input read, each output written once), so it is shaped like a
 // copy: one unit of work a thread, no loop, no shared memory, few registers, the data on its way
 // before the token's place is looked up. A unit is two vectors (of 16 bytes where everything is
-// aligned) of one head: V pairs of a rotated head, or what is copied as it is. Threads that keep the
-// angles for several heads or tokens were slower (8 contexts of 3392 tokens, 16 + 8 heads of 128:
-// 79 to 114 us against 78 us, 5.7 TB/s), for want of loads in flight; at 40 registers 12 blocks of 128
-// threads are resident.
+// aligned) of one head: V pairs of a rotated head, or what is copied as it is. At 40 registers 12 blocks
+// of 128 threads are resident. 8 contexts of 3392 tokens, 16 + 8 heads of 128, take 70 us (6.3 TB/s, 98%
+// of the measured copy rate). With hardware divisions it was 78 us, bound by instruction issue; threads
+// that kept the angles for several heads or tokens took 79 to 114 us, for want of loads in flight.
 // ---------------------------------------------------------------------------------------------
 constexpr int kAppendThreads = 128;
 
@@ -510,6 +510,10 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_plain_kernel(const AttnA
 // row (values 8j.. of each 32) is the A fragment of two steps, with Q held in the same order. V is
 // read transposed by ldmatrix. Weights leave the S^T fragments for the P^T ones by an 8 x 8 transpose
 // in registers, and each head's maximum and sum live in the lanes that hold its columns of O^T.
+//
+// 64 sequences of 3392 tokens, 16 query and 8 key heads of 128, take 137 us (6.45 TB/s, the measured
+// copy rate); with lengths spread from 0 up 75 us (5.9 TB/s), the rest being the kernel's start, its
+// tail and the join; one sequence of 131001 tokens 89 us (6.05 TB/s).
 //
 // The weights p = exp(z - m) would lose 8 bits (bf16) as an operand, so they go in as two: hi, p
 // rounded a little low so that p - hi > 0, and the rest; one step is two products, 2^-16 of p is left
@@ -1101,10 +1105,11 @@ int launch_attn(const AttnArgs& a, bool mma, cudaStream_t st) {
 
 // The split of a call into units and CTAs; false where positions of the list would not fit 31 bits.
 // Short caches (up to 48 tiles a sequence): one CTA for each (sequence, unit), one launch (400 tokens,
-// 8 sequences of 8 key heads of 128: 7.6 us, divided 10 us; 1000 tokens, 4 sequences: 12.4 us, divided
-// 10 us). Else the list is divided over as many CTAs as the GPU holds; where there is much work for
-// each of them, they take 80% of it and as many smaller runs follow (64 ragged sequences of up to 3392:
-// 75 us against 84; all of 3392: 137 us against 140).
+// 8 sequences of 8 key heads of 128: 7.7 us, divided 9.8 us; 300 sequences of up to 500: 53 us against
+// 89 us; but 1000 tokens, 4 sequences: 12.5 us, divided 9.8 us). Else the list is divided over as many
+// CTAs as the GPU holds; where there is much work for each of them, they take 80% of it and as many
+// smaller runs follow (64 ragged sequences of up to 3392: 75 us against 84; all of 3392: 138 us against
+// 139; 16 of 6000, 8 heads of 96: 62 us against 69).
 bool plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool mma, int sms, AttnArgs& a) {
   a.B = (int)B;
   a.Hq = (int)Hq;
