@@ -192,13 +192,16 @@ __global__ void __launch_bounds__(kAppendThreads, 12) append_kernel(const Append
 // a sequence of length 0 gives a row of zeros.
 //
 // Work split. The work is the list of (sequence, unit, tile of 16 tokens) in that order, a unit
-// being one key head with a block of its query heads. The kernel's CTAs divide the
-// list into equal runs, so a batch of ragged lengths is as balanced as one long sequence, with no
-// knowledge of the lengths on the host: each CTA finds its first sequence with a warp scan over the
-// lengths. A (sequence, unit) covered by one CTA is finished there; where several CTAs share it,
+// being one key head with a block of its query heads. The kernel's CTAs divide the list into runs that
+// do not care where sequences end, so a batch of ragged lengths is as balanced as one long sequence,
+// with no knowledge of the lengths on the host: each CTA finds its first sequence with a warp scan over
+// the lengths. A (sequence, unit) covered by one CTA is finished there; where several CTAs share it,
 // each leaves its running maximum, sum and unnormalised fp32 output in a slot of the workspace (at
 // most two slots a CTA: its first and its last run), and attn_join_kernel combines them in the
 // order of the list, so results do not depend on timing.
+//
+// Where there are many (sequence, unit) pairs, each has a CTA of its own for its first `head` tiles
+// (no search, no shared rows as long as that is all), and the list holds what lies behind them.
 // ---------------------------------------------------------------------------------------------
 constexpr int kTile = 16;
 constexpr int kAttnWarps = 4;
@@ -209,12 +212,12 @@ struct AttnArgs {
   const void *q, *k_cache, *v_cache;
   void* out;
   const int32_t *table, *lengths;
-  float *ws_o, *ws_ml;  // [2 * ctas][rows][D] and [2 * ctas][rows][2]
+  float *ws_o, *ws_ml;  // [2 * (mains + ctas)][rows][D] and [2 * (mains + ctas)][rows][2]
   uint32_t* status;
   int B, Hq, Hkv, D, G;        // G = Hq / Hkv query heads per key head
   int rows, subs, units;       // query heads a unit covers; units per key head; units per sequence
-  int whole;                   // one CTA for each (sequence, unit): nothing is shared
-  int ctas, big, min_tiles;    // CTAs, and how many of them take the larger runs
+  int mains, head;             // CTAs that each have the first `head` tiles of a (sequence, unit), or 0, 0
+  int ctas, big, min_tiles;    // CTAs that divide the list, and how many of them take the larger runs
   float share;                 // of the list that those take
   int cap;                     // tokens that a row of the table has room for
   int page_size, n_pages, table_width;
@@ -231,6 +234,8 @@ __device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
   return n;
 }
 __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+// Tiles of a sequence that are in the list.
+__device__ __forceinline__ int listed_tiles(const AttnArgs& a, int len) { return max(0, tiles_of(len) - a.head); }
 
 // The list's division (positions fit 31 bits: the host sees to it): the first `big` CTAs take `per`
 // tiles each, the others, which start as those end, `small` tiles. SMs do not run at one speed (the
@@ -244,7 +249,7 @@ struct Division {
       per = max(a.min_tiles, (int)(((uint32_t)total + a.ctas - 1) / (uint32_t)a.ctas));
       small = 1;
     } else {
-      per = max(a.min_tiles, (int)((float)total * a.share) / big + 1);
+      per = max(a.min_tiles, (int)((float)total * a.share / (float)big) + 1);
       const int left = total - (int)min((int64_t)total, (int64_t)per * big);
       small = max(a.min_tiles, (int)(((uint32_t)left + rest - 1) / (uint32_t)rest));
     }
@@ -260,7 +265,7 @@ struct Division {
 };
 
 // Where a CTA's run begins: the sequence that holds its first position, that sequence's length and the
-// tiles before it; false where the list ends before. Warp-collective; the lengths of up to 128
+// listed tiles before it; false where the list ends before. Warp-collective; the lengths of up to 128
 // sequences are read once, of more twice.
 struct Start { int pos, size, total, b, len, before; };
 __device__ __forceinline__ bool find_start(const AttnArgs& a, int cta, Start& st) {
@@ -271,8 +276,8 @@ __device__ __forceinline__ bool find_start(const AttnArgs& a, int cta, Start& st
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < a.B ? seq_len(a, 32 * i + lane) : 0;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) all += tiles_of(held[i]);
-  for (int s = 32 * kHeld + lane; s < a.B; s += 32) all += tiles_of(seq_len(a, s));
+  for (int i = 0; i < kHeld; ++i) all += listed_tiles(a, held[i]);
+  for (int s = 32 * kHeld + lane; s < a.B; s += 32) all += listed_tiles(a, seq_len(a, s));
   st.total = (int)__reduce_add_sync(0xffffffffu, all) * a.units;
   const Division div(a, st.total);
   const int64_t pos = div.begin(cta);
@@ -286,7 +291,7 @@ __device__ __forceinline__ bool find_start(const AttnArgs& a, int cta, Start& st
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) len = base == 32 * i ? held[i] : len;
     if (base >= 32 * kHeld) len = base + lane < a.B ? seq_len(a, base + lane) : 0;
-    const int mine = tiles_of(len);
+    const int mine = listed_tiles(a, len);
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -312,40 +317,45 @@ struct Parts {
   int b, kvh, row0, rows;  // sequence, key head, first query head and number of query heads
   int tile0, tile1, len;
   int slot;                // workspace slot, or -1: the CTA covers all of the unit and finishes its rows
-  int unit, tiles;
+  int unit, tiles;         // tiles: of the sequence, in the list
   int left;                // tiles of the run behind this part
 
-  __device__ __forceinline__ void set(const AttnArgs& a, int tile, int free_slot) {
+  __device__ __forceinline__ void set_heads(const AttnArgs& a) {
     kvh = unit / a.subs;
     const int sub = unit - kvh * a.subs;
     row0 = kvh * a.G + sub * a.rows;
     rows = min(a.rows, a.G - sub * a.rows);
+  }
+  __device__ __forceinline__ void set(const AttnArgs& a, int tile, int free_slot) {
+    set_heads(a);
     const int n = min(tiles - tile, left);
-    tile0 = tile;
-    tile1 = tile + n;
+    tile0 = a.head + tile;
+    tile1 = tile0 + n;
     left -= n;
-    slot = n == tiles ? -1 : free_slot;
+    // all of the listed tiles: the unit is finished, or (its head being elsewhere) has a slot by its number
+    slot = n < tiles ? a.mains + free_slot : a.head == 0 ? -1 : a.mains + 2 * a.ctas + b * a.units + unit;
   }
   // False: the CTA has nothing to do. (All warps of the CTA compute the same.)
   __device__ __forceinline__ bool first(const AttnArgs& a) {
-    if (a.whole) {
+    if ((int)blockIdx.x < a.mains) {
       b = blockIdx.x / a.units;
       unit = blockIdx.x - b * a.units;
+      set_heads(a);
       len = seq_len(a, b);
-      tiles = tiles_of(len);
-      left = tiles;
-      set(a, 0, -1);
+      left = tile0 = 0;
+      tile1 = min(tiles_of(len), a.head);
+      slot = tiles_of(len) > a.head ? (int)blockIdx.x : -1;
       return len > 0;
     }
     Start st;
-    if (!find_start(a, blockIdx.x, st)) return false;
+    if (!find_start(a, blockIdx.x - a.mains, st)) return false;
     left = st.size;
     b = st.b;
     len = st.len;
-    tiles = tiles_of(len);
+    tiles = listed_tiles(a, len);
     const int off = st.pos - st.before * a.units;
     unit = (int)((uint32_t)off / (uint32_t)tiles);
-    set(a, off - unit * tiles, 2 * blockIdx.x);
+    set(a, off - unit * tiles, 2 * (blockIdx.x - a.mains));
     return true;
   }
   __device__ __forceinline__ bool next(const AttnArgs& a) {
@@ -355,10 +365,10 @@ struct Parts {
       do {
         ++b;
         len = seq_len(a, b);
-      } while (len == 0);
-      tiles = tiles_of(len);
+        tiles = listed_tiles(a, len);
+      } while (tiles == 0);
     }
-    set(a, 0, 2 * blockIdx.x + 1);
+    set(a, 0, 2 * (blockIdx.x - a.mains) + 1);
     return true;
   }
 };
@@ -909,25 +919,35 @@ __global__ void __launch_bounds__(NT) attn_join_kernel(const AttnArgs a) {
   __shared__ alignas(16) float s_acc[NT * VEC];
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq;
   const int kvh = h / a.G, sub = (h - kvh * a.G) / a.rows, g = h - kvh * a.G - sub * a.rows;
-  const int tiles = tiles_of(seq_len(a, b));
-  uint32_t sum_before = 0, sum_all = 0;
+  const int tiles = listed_tiles(a, seq_len(a, b));
+  int c0 = 0, c1 = 0, first = 0;
+  if (tiles > 0) {
+    uint32_t sum_before = 0, sum_all = 0;
 #pragma unroll 4
-  for (int i = threadIdx.x & 31; i < a.B; i += 32) {
-    const int t = tiles_of(seq_len(a, i));
-    sum_all += t;
-    sum_before += i < b ? t : 0;
+    for (int i = threadIdx.x & 31; i < a.B; i += 32) {
+      const int t = listed_tiles(a, seq_len(a, i));
+      sum_all += t;
+      sum_before += i < b ? t : 0;
+    }
+    const int total = (int)__reduce_add_sync(0xffffffffu, sum_all) * a.units;
+    const Division div(a, total);
+    const int s0 = (int)__reduce_add_sync(0xffffffffu, sum_before) * a.units + (kvh * a.subs + sub) * tiles;
+    c0 = div.cta_of(s0);
+    c1 = div.cta_of(s0 + tiles - 1);
+    // the first CTA has the rows in its last slot unless its run starts there
+    first = 2 * c0 + (div.begin(c0) < s0 ? 1 : 0);
   }
-  const int total = (int)__reduce_add_sync(0xffffffffu, sum_all) * a.units;
-  const Division div(a, total);
-  const int s0 = (int)__reduce_add_sync(0xffffffffu, sum_before) * a.units + (kvh * a.subs + sub) * tiles, s1 = s0 + tiles;
-  const int c0 = tiles ? div.cta_of(s0) : 0, c1 = tiles ? div.cta_of(s1 - 1) : 0;
   // launched while the main kernel still runs; its parts are complete behind this point
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c0 == c1) return;  // empty, or finished by the one CTA that had it
-  // the first CTA has the rows in its last slot unless its run starts there
-  const int first = 2 * c0 + (div.begin(c0) < s0 ? 1 : 0);
-  auto row_of = [&](int i) { return (int64_t)(i == 0 ? first : 2 * (c0 + i)) * a.rows + g; };
-  const int n = c1 - c0 + 1;
+  if (tiles == 0 || (a.head == 0 && c0 == c1)) return;  // finished by the one CTA that had it, or empty
+  const int heads = a.head > 0 ? 1 : 0, pair = b * a.units + kvh * a.subs + sub;  // parts in front of the list's
+  auto row_of = [&](int i) {
+    const int slot = i < heads              ? pair
+                     : heads == 1 && c0 == c1 ? a.mains + 2 * a.ctas + pair
+                                              : a.mains + (i == heads ? first : 2 * (c0 + i - heads));
+    return (int64_t)slot * a.rows + g;
+  };
+  const int n = heads + c1 - c0 + 1;
   const int lanes = (a.D + VEC - 1) / VEC, warp = threadIdx.x >> 5;
   const int nway = lanes >= NT ? 1 : NT / lanes;
   const int way = threadIdx.x / lanes, d = (threadIdx.x - way * lanes) * VEC;
@@ -1037,8 +1057,8 @@ int launch_append(AppendArgs& a, cudaStream_t st) {
 
 template <typename T, int DP>
 int launch_plain(const AttnArgs& a, cudaStream_t st) {
-  if (a.rows == 1) attn_plain_kernel<T, DP, 1><<<a.ctas, 32 * kAttnWarps, 0, st>>>(a);
-  else attn_plain_kernel<T, DP, 4><<<a.ctas, 32 * kAttnWarps, 0, st>>>(a);
+  if (a.rows == 1) attn_plain_kernel<T, DP, 1><<<a.mains + a.ctas, 32 * kAttnWarps, 0, st>>>(a);
+  else attn_plain_kernel<T, DP, 4><<<a.mains + a.ctas, 32 * kAttnWarps, 0, st>>>(a);
   return (int)cudaGetLastError();
 }
 
@@ -1053,7 +1073,7 @@ int launch_mma_one(const AttnArgs& a, cudaStream_t st) {
     if (e == cudaSuccess && dev < 64) ready |= 1ull << dev;
   }
   if (e != cudaSuccess) return (int)e;
-  attn_mma_kernel<T, D, NG, PAGE16><<<a.ctas, 32 * kAttnWarps, kSmem, st>>>(a);
+  attn_mma_kernel<T, D, NG, PAGE16><<<a.mains + a.ctas, 32 * kAttnWarps, kSmem, st>>>(a);
   return (int)cudaGetLastError();
 }
 
@@ -1096,20 +1116,21 @@ int launch_attn(const AttnArgs& a, bool mma, cudaStream_t st) {
     else if (a.D <= 128) rc = launch_plain<T, 4>(a, st);
     else rc = launch_plain<T, 8>(a, st);
   }
-  if (rc != 0 || a.whole || a.ctas == 1) return rc;  // nothing to join
+  if (rc != 0 || a.ctas == 0 || (a.mains == 0 && a.ctas == 1)) return rc;  // nothing to join
   // (the second threshold: one long sequence has tens of parts a head)
-  const bool vec = a.D % 4 == 0 && aligned16(a.ws_o), wide = a.ctas >= 16 * a.B * a.units;
+  const bool vec = a.D % 4 == 0 && aligned16(a.ws_o), wide = a.ctas >= 16 * (int64_t)a.B * a.units;
   if (vec) return wide ? launch_join<T, 4, 512>(a, st) : launch_join<T, 4, 128>(a, st);
   return launch_join<T, 1, 128>(a, st);
 }
 
 // The split of a call into units and CTAs; false where positions of the list would not fit 31 bits.
-// Short caches (up to 48 tiles a sequence): one CTA for each (sequence, unit), one launch (400 tokens,
-// 8 sequences of 8 key heads of 128: 7.7 us, divided 9.8 us; 300 sequences of up to 500: 53 us against
-// 89 us; but 1000 tokens, 4 sequences: 12.5 us, divided 9.8 us). Else the list is divided over as many
-// CTAs as the GPU holds; where there is much work for each of them, they take 80% of it and as many
-// smaller runs follow (64 ragged sequences of up to 3392: 75 us against 84; all of 3392: 138 us against
-// 139; 16 of 6000, 8 heads of 96: 62 us against 69).
+// Many (sequence, unit) pairs: one CTA for each with up to 8192 tokens, the list for the rest (512 ragged
+// sequences of up to 2000: 295 us, 7.1 TB/s, divided 366 us; 256 of up to 3000: 227 us against 263 us; one
+// of 60000 among 255 of up to 1000: 145 us against 137 us). The same for short caches, up to 48 tiles a sequence, however few (400 tokens, 8 sequences of 8 key heads
+// of 128: 7.7 us, divided 9.8 us; but 1000 tokens, 4 sequences: 12.5 us, divided 9.8 us). Else the list
+// is divided over as many CTAs as the GPU holds; where there is much work for each of them, they take
+// 80% of it and as many smaller runs follow (64 ragged sequences of up to 3392: 75 us against 84; all of
+// 3392: 138 us against 139; 16 of 6000, 8 heads of 96: 62 us against 69).
 bool plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool mma, int sms, AttnArgs& a) {
   a.B = (int)B;
   a.Hq = (int)Hq;
@@ -1127,12 +1148,16 @@ bool plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool 
   a.cap = (int)(capacity < INT_MAX - 2 * kTile ? capacity : INT_MAX - 2 * kTile);
   const int64_t pairs = B * a.units, per_seq = (a.cap + kTile - 1) / kTile;
   const int64_t slots = (int64_t)sms * (mma ? attn_ctas(a.D, a.rows <= 8 ? 1 : 2) : 4);
+  constexpr int kHead = 512;
   a.min_tiles = kAttnWarps;
   a.share = 0.f;
-  a.whole = per_seq <= 48 && pairs <= INT_MAX;
-  if (a.whole) {
-    a.ctas = a.big = (int)pairs;
-    return true;
+  a.mains = a.head = 0;
+  const bool few_tiles = per_seq <= 48;
+  if (few_tiles || (pairs >= 4 * slots && (per_seq <= kHead || pairs * a.rows * (D + 2) * 8 <= (64 << 20)))) {
+    a.mains = (int)pairs;
+    a.head = few_tiles ? 48 : kHead;
+    a.ctas = a.big = per_seq <= a.head ? 0 : (int)slots;
+    return pairs <= INT_MAX - slots && (a.ctas == 0 || per_seq * pairs <= INT_MAX);
   }
   if (per_seq * pairs > INT_MAX) return false;
   const int64_t want = (pairs * per_seq + a.min_tiles - 1) / a.min_tiles;
@@ -1146,7 +1171,7 @@ bool plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool 
   return true;
 }
 
-int64_t ws_floats(const AttnArgs& a) { return a.whole ? 0 : (int64_t)2 * a.ctas * a.rows * (a.D + 2); }
+int64_t ws_floats(const AttnArgs& a) { return a.ctas == 0 ? 0 : 2 * ((int64_t)a.mains + a.ctas) * a.rows * (a.D + 2); }
 
 }  // namespace
 
@@ -1219,7 +1244,7 @@ NFB_API int nfb_paged_attn(int dtype, const void* q, const void* k_cache, const 
   a.page_size = (int)dims[4]; a.n_pages = (int)dims[5]; a.table_width = (int)dims[6];
   a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.out = out; a.table = table; a.lengths = lengths;
   a.ws_o = ws;
-  a.ws_ml = ws + (int64_t)2 * a.ctas * a.rows * D;
+  a.ws_ml = ws + 2 * ((int64_t)a.mains + a.ctas) * a.rows * D;
   a.status = status;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.q_sb = dims[7]; a.q_sh = dims[8]; a.o_sb = dims[9]; a.o_sh = dims[10];

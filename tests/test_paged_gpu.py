@@ -119,6 +119,27 @@ def test_attention_long_and_many_sequences(dtype, B, hq, hk, d, L):
         assert torch.equal(out, paged_attention(q, kc, vc, table, lengths))
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("longest", [500, 8192, 70000])
+def test_attention_many_sequences_and_a_few_long_ones(dtype, d, longest):
+    """More (sequence, head) pairs than the GPU holds: each has a block for its first 8192 tokens, and what lies
+    behind them is divided. Sequences share pages here (a table may name a page more than once)."""
+    g = _gen(longest + d)
+    B, ps, pages = 300, 64, 300
+    kc, vc = _pool(pages, ps, 8, d, dtype, g)
+    W = -(-longest // ps)
+    table = torch.randint(0, pages, (B, W), generator=g, device=DEV, dtype=torch.int32)
+    lengths = torch.randint(0, min(longest, 90), (B,), generator=g, device=DEV, dtype=torch.int32)
+    for i, n in enumerate((longest, 8191, 8192, 8193, 8208, 8209, 12345, 0, 1, longest)):
+        lengths[29 * i] = min(n, longest)
+    q = torch.randn(B, 1, 16, d, generator=g, device=DEV).to(dtype)
+    out = paged_attention(q, kc, vc, table, lengths)
+    _check_attention(out, q, kc, vc, table, lengths)
+    assert torch.equal(out, paged_attention(q, kc, vc, table, lengths))
+    lengths.clamp_(max=5)                             # the same table, only short sequences
+    _check_attention(paged_attention(q, kc, vc, table, lengths), q, kc, vc, table, lengths)
+
+
 def test_attention_large_scores_and_custom_scale():
     """Scores of several hundred: the weights collapse to one token; a growing maximum rescales the sums."""
     g = _gen(5)
