@@ -1126,11 +1126,12 @@ int launch_attn(const AttnArgs& a, bool mma, cudaStream_t st) {
 // The split of a call into units and CTAs; false where positions of the list would not fit 31 bits.
 // Many (sequence, unit) pairs: one CTA for each with up to 8192 tokens, the list for the rest (512 ragged
 // sequences of up to 2000: 295 us, 7.1 TB/s, divided 366 us; 256 of up to 3000: 227 us against 263 us; one
-// of 60000 among 255 of up to 1000: 145 us against 137 us). The same for short caches, up to 48 tiles a sequence, however few (400 tokens, 8 sequences of 8 key heads
-// of 128: 7.7 us, divided 9.8 us; but 1000 tokens, 4 sequences: 12.5 us, divided 9.8 us). Else the list
-// is divided over as many CTAs as the GPU holds; where there is much work for each of them, they take
-// 80% of it and as many smaller runs follow (64 ragged sequences of up to 3392: 75 us against 84; all of
-// 3392: 138 us against 139; 16 of 6000, 8 heads of 96: 62 us against 69).
+// of 60000 among 255 of up to 1000: 145 us against 137 us). The same for short caches, up to 48 tiles a
+// sequence, however few (400 tokens, 8 sequences of 8 key heads of 128: 7.7 us, divided 9.8 us; but 1000
+// tokens, 4 sequences: 12.5 us, divided 9.8 us). Else the list is divided over as many CTAs as the GPU
+// holds; where there is much work for each of them, they take 80% of it and as many smaller runs follow
+// (64 ragged sequences of up to 3392: 75 us against 84; all of 3392: 138 us against 139; 16 of 6000, 8
+// heads of 96: 62 us against 69).
 bool plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity, bool mma, int sms, AttnArgs& a) {
   a.B = (int)B;
   a.Hq = (int)Hq;
