@@ -1,14 +1,16 @@
 // Log probabilities of given tokens, the entropy of each row and its most likely tokens, from
 // materialised logits, with the gradient.
 //
-// With m = max_j z_j, s = sum_j exp(z_j - m), u = sum_j exp(z_j - m) (z_j - m):
-//   log p_t = (z_t - m) - log s,   H = -sum_j p_j log p_j = log s - u / s,
+// With m = max_j z_j, r = sum of exp(z_j - m) over all j but one that has the maximum, and
+// u = sum_j exp(z_j - m) (z_j - m):
+//   log p_t = (z_t - m) - log(1 + r),   H = -sum_j p_j log p_j = log(1 + r) - u / (1 + r),
 // so one pass over a row with a running maximum and sums gives both; a masked logit (-inf) adds
-// nothing to either sum. The alternatives are the top_k largest logits, equal ones in the order of
-// their index. The gradient of g log p_t + e H + sum_i a_i log p_{k_i} is
+// nothing to either sum. The sum is kept as its excess over 1 because a trained head often has a
+// row's mass on one token: then log p_t = -r + ..., and a sum near 1 would have lost the digits of r.
+// The alternatives are the top_k largest logits, equal ones in the order of their index. The gradient
+// of g log p_t + e H + sum_i a_i log p_{k_i} is
 //   dz_j = -p_j (g + sum_i a_i + e (log p_j + H)) + g [j = t] + sum_i a_i [j = k_i].
-// Sums and statistics are fp32; m and s are kept apart for the backward pass, since their sum
-// m + log s would round away the low bits of log s.
+// Sums and statistics are fp32; m and r are kept apart for the backward pass.
 #include <climits>
 #include <cooperative_groups.h>
 
@@ -25,7 +27,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 struct LpArgs {
   const void* logits;
   const int64_t* targets;  // null: none
-  float *logprobs, *entropy, *stats;  // stats: (m, s) of each row, or null
+  float *logprobs, *entropy, *stats;  // stats: (m, r) of each row, or null
   float* top_logprobs;
   int64_t* top_tokens;
   uint32_t* status;
@@ -34,6 +36,7 @@ struct LpArgs {
 };
 
 struct Stat { float m, s, u; };  // maximum; sums of exp(z - m) and of exp(z - m) (z - m)
+struct RowStat { float m, r, u; };  // the same with r = s - 1; r = -1: no finite logit
 
 // z - m clamped so that a masked logit gives 0 * finite, not 0 * inf; NaN passes through. (The
 // difference is taken before the factor log2(e): a row at the type's lowest value stays finite.)
@@ -54,11 +57,15 @@ __device__ __forceinline__ Stat stat_at(Stat a, float m) {
   const float c = below_max(a.m, or_zero(m)), e = exp_of(c);
   return {m, a.s * e, e * (a.u + a.s * c)};
 }
-__device__ __forceinline__ Stat stat_merge(Stat a, Stat b) {
-  const float m = fmaxf(a.m, b.m);
-  a = stat_at(a, m);
-  b = stat_at(b, m);
-  return {m, a.s + b.s, a.u + b.u};
+// The statistics of two disjoint parts of a row together.
+__device__ __forceinline__ RowStat row_merge(RowStat a, RowStat b) {
+  if (b.m > a.m) {
+    const RowStat t = a;
+    a = b;
+    b = t;
+  }
+  const float c = below_max(b.m, or_zero(a.m)), e = exp_of(c), s = 1.f + b.r;
+  return {a.m, a.r + s * e, a.u + e * (b.u + s * c)};
 }
 
 // Order of the alternatives as one number: the value (zeros of both signs alike), then the lower index.
@@ -135,7 +142,7 @@ __device__ __forceinline__ float kth_of_warp(float v, int k) {
 //
 // What bounds it: for 16-bit logits the HBM's rate leaves 11 issue slots of an SM for a warp's 32 values,
 // and the sums take 8 with one exponential among them. Without alternatives 16384 x 32000 bf16 take
-// 173 us (6.05 TB/s, 94% of the measured copy rate); with 5 the issue slots bind (84% busy): 224 us.
+// 178 us (5.9 TB/s, 92% of the measured copy rate); with 5 the issue slots bind (84% busy): 229 us.
 constexpr int kLpUnroll = 4, kLpAbove = 512, kLpEqual = 128;
 
 template <typename T, int NT>
@@ -149,7 +156,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
   __shared__ uint64_t s_cand[kLpAbove + kLpEqual];
   __shared__ uint64_t s_best[kMaxTop];        // keys of the alternatives, descending; 0: none
   __shared__ uint64_t s_round[kWarps];
-  __shared__ Stat s_row;
+  __shared__ RowStat s_row;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = a.split == 1 ? blockIdx.x : blockIdx.x / a.split;
   const int rank = a.split == 1 ? 0 : blockIdx.x % a.split;
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     st.s += s;
     st.u += u;
   }
-  // the warps' sums, then the row's by warp 1 while the others rank
+  // the warps' sums, then the row's by the warp that has the maximum
   {
     Stat t = stat_at(st, warp_max(st.m));
     t.s = warp_sum(t.s);
@@ -246,12 +253,38 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
   }
   if (k > 0) publish(mx);
   __syncthreads();
-  if (warp == 1) {
+  {
     Stat t = lane < kWarps ? s_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-    t = stat_at(t, warp_max(t.m));
-    t.s = warp_sum(t.s);
-    t.u = warp_sum(t.u);
-    if (lane == 0) s_row = t;
+    const float m = warp_max(t.m);
+    const int owner = __ffs(__ballot_sync(0xffffffffu, t.m == m)) - 1;
+    if (warp == owner) {
+      t = stat_at(t, m);
+      const float sum = warp_sum(t.s), u = warp_sum(t.u);
+      float r = sum - 1.f;
+      if (sum < 2.f && m != -INFINITY) {
+        // the sum may be little more than 1: everything but the maximum again, by whole warps where that
+        // is exact enough, and value by value (a lane each) for the thread that has the maximum
+        const int src = __ffs(__ballot_sync(0xffffffffu, mx == m)) - 1, src_tid = tid - lane + src;
+        r = (lane < kWarps && lane != owner ? t.s : 0.f) + (lane != src ? stat_at(st, m).s : 0.f);
+        const int n = max(0, (last - first - src_tid + NT - 1) / NT) * VE;
+        bool left_out = false;
+#pragma unroll 4
+        for (int e0 = 0; e0 < n; e0 += 32) {
+          const int e = e0 + lane;
+          const float z = e < n ? to_f32(x[head + (first + src_tid + e / VE * NT) * VE + e % VE]) : -INFINITY;
+          const uint32_t hit = __ballot_sync(0xffffffffu, z == m);
+          if (e < n && (left_out || lane != __ffs(hit) - 1)) r += exp_of(below_max(z, m));
+          left_out = left_out || hit != 0;
+        }
+        const int one = __shfl_sync(0xffffffffu, single, src);
+        if (one >= 0 && lane == 0) {
+          const float z = to_f32(x[one]);
+          if (left_out || z != m) r += exp_of(below_max(z, m));
+        }
+        r = warp_sum(r);
+      }
+      if (lane == 0) s_row = {m, r, u};
+    }
   }
   auto rank_in = [&](const uint64_t* list, int n, uint64_t mine) {
     int better = 0;
@@ -355,12 +388,12 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     }
   }
   __syncthreads();
-  Stat t = s_row;
+  RowStat t = s_row;
   if (a.split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (rank == 0 && warp == 0) {
-      for (int r = 1; r < a.split; ++r) t = stat_merge(t, *cluster.map_shared_rank(&s_row, r));
+      for (int r = 1; r < a.split; ++r) t = row_merge(t, *cluster.map_shared_rank(&s_row, r));
       if (k > 0) {  // the CTAs' lists, ranked again
         for (int r = 0; r < a.split; ++r)
           if (lane < k) s_cand[r * k + lane] = cluster.map_shared_rank(s_best, r)[lane];
@@ -380,14 +413,14 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
     if (rank != 0) return;
   }
   if (warp != 0) return;
-  const float m = or_zero(t.m), log_s = logf(t.s);
+  const float m = or_zero(t.m), log_s = log1pf(t.r);
+  const bool none = t.r == -1.f;  // no finite logit: no distribution, its entropy is 0
   if (lane == 0) {
     if (a.stats) {
       a.stats[2 * row] = m;
-      a.stats[2 * row + 1] = t.s;
+      a.stats[2 * row + 1] = t.r;
     }
-    // a row without a finite logit has no distribution: its entropy is 0
-    a.entropy[row] = t.s == 0.f ? 0.f : log_s - t.u / t.s;
+    a.entropy[row] = none ? 0.f : log_s - t.u / (1.f + t.r);
     if (a.targets) {
       const int64_t j = a.targets[row];
       float lp = 0.f;
@@ -396,7 +429,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
           set_status(a.status, kBadArgument, kSiteTarget);
           lp = __int_as_float(0x7fffffff);
         } else {
-          lp = t.s == 0.f ? -INFINITY : (to_f32(x[j]) - m) - log_s;
+          lp = none ? -INFINITY : (to_f32(x[j]) - m) - log_s;
         }
       }
       a.logprobs[row] = lp;
@@ -405,7 +438,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_kernel(const LpArgs a)
   if (lane < k) {
     const uint64_t key = s_best[lane];  // 0: only a row with NaN runs out of values
     a.top_tokens[row * k + lane] = key == 0 ? 0 : (int)~(uint32_t)key;
-    a.top_logprobs[row * k + lane] = t.s == 0.f ? -INFINITY : (key_value(key) - m) - log_s;
+    a.top_logprobs[row * k + lane] = none ? -INFINITY : (key_value(key) - m) - log_s;
   }
 }
 
@@ -420,85 +453,108 @@ struct LpBwdArgs {
 };
 
 // Backward: a stream over the row, bound by its bytes (each logit read, each gradient written: 16384 x
-// 32000 bf16 in 325 us, the measured copy rate). With
-// d = z - m the gradient apart from the given tokens is exp(d) (c1 d + c0), c0 and c1 of the row. The
-// given tokens' places are written again by the first threads, each with its whole value (a token may
-// be the target and an alternative), rounded once.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) logprobs_bwd_kernel(const LpBwdArgs a) {
+// 32000 bf16 in 312 us, 6.7 TB/s, the measured copy rate). With d = z - m the gradient apart from the
+// given tokens is exp(d) (c1 d + c0), c0 and c1 of the row, which one warp prepares while the first
+// logits are on their way. The given tokens' places are written
+// again by the first threads, each with its whole value (a token may be the target and an alternative),
+// rounded once.
+// 40 registers: 16384 x 32000 bf16 312 us; 32 and a spill 321 us, 48 320 us, 64 349 us (fewer CTAs).
+template <typename T, int NT, bool VEC>
+__global__ void __launch_bounds__(NT, 1536 / NT) logprobs_bwd_kernel(const LpBwdArgs a) {
   constexpr int VE = 16 / sizeof(T), kVecs = 4;
   __shared__ int s_idx[kMaxTop + 1];
   __shared__ float s_g[kMaxTop + 1];
+  __shared__ float s_c0, s_c1, s_log;
   const int64_t row = blockIdx.x / a.chunks;
   const int chunk = (int)(blockIdx.x - row * a.chunks);
   const T* x = (const T*)a.logits + row * a.ld;
   T* dx = (T*)a.d_logits + row * a.V;
-  const int n_fix = a.top_k + 1;
-  if ((int)threadIdx.x < n_fix) {  // entry 0: the target; then the alternatives
-    int j = -1;
-    float g = 0.f;
-    if (threadIdx.x == 0) {
-      if (a.g_logprobs) {
-        const int64_t t = a.targets[row];
-        if (t != a.ignore_index && t >= 0 && t < a.V) {
-          j = (int)t;
-          g = a.g_logprobs[row];
-        }
-      }
-    } else if (a.g_top) {
-      j = (int)a.top_tokens[row * a.top_k + threadIdx.x - 1];
-      g = a.g_top[row * a.top_k + threadIdx.x - 1];
-    }
-    s_idx[threadIdx.x] = j;
-    s_g[threadIdx.x] = g;
+  const int begin = chunk * a.per, end = min(a.V, begin + a.per);
+  // VEC: x and dx begin at the same distance from a 16-byte boundary
+  const int head = VEC ? min(end, begin + (int)((-reinterpret_cast<uintptr_t>(x + begin) & 15) / sizeof(T))) : end;
+  const int vecs = (end - head) / VE, tail = head + vecs * VE;
+  uint4 w[kVecs];
+  if constexpr (VEC) {
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if ((int)threadIdx.x + i * NT < vecs) w[i] = __ldcs(xv + threadIdx.x + i * NT);
   }
-  const float m = a.stats[2 * row], s = a.stats[2 * row + 1], log_s = logf(s);
+  const float m = a.stats[2 * row], r = a.stats[2 * row + 1];
   const float e = a.g_entropy ? a.g_entropy[row] : 0.f, H = a.entropy[row];
-  const float inv = s == 0.f ? 0.f : 1.f / s;
+  const bool none = r == -1.f;  // no finite logit: no gradient
+  const float inv = none ? 0.f : 1.f / (1.f + r);
+  const int n_fix = a.top_k + 1;
+  if (threadIdx.x < 32) {
+    // entry 0: the target; then the alternatives
+    float whole = 0.f;
+    for (int i = threadIdx.x; i < n_fix; i += 32) {
+      int j = -1;
+      float g = 0.f;
+      if (i == 0) {
+        if (a.g_logprobs) {
+          const int64_t t = a.targets[row];
+          if (t != a.ignore_index && t >= 0 && t < a.V) {
+            j = (int)t;
+            g = a.g_logprobs[row];
+          }
+        }
+      } else if (a.g_top) {
+        j = (int)a.top_tokens[row * a.top_k + i - 1];
+        g = a.g_top[row * a.top_k + i - 1];
+      }
+      s_idx[i] = j;
+      s_g[i] = g;
+      whole += g;
+    }
+    whole = warp_sum(whole);
+    if (threadIdx.x == 0) {
+      const float log_s = log1pf(r);
+      s_log = log_s;
+      s_c0 = none ? 0.f : -(whole + e * (H - log_s)) * inv;
+      s_c1 = -e * inv;
+    }
+  }
   __syncthreads();
-  float whole = 0.f;
-  for (int i = 0; i < n_fix; ++i) whole += s_g[i];
-  // a row without a finite logit has s = 0: no gradient
-  const float c0 = s == 0.f ? 0.f : -(whole + e * (H - log_s)) * inv, c1 = -e * inv;
+  const float c0 = s_c0, c1 = s_c1, log_s = s_log;
   auto grad = [&](float z) {
     const float d = below_max(z, m);
     return exp_of(d) * fmaf(c1, d, c0);
   };
-  const int begin = chunk * a.per, end = min(a.V, begin + a.per);
   if constexpr (VEC) {
-    // x and dx begin at the same distance from a 16-byte boundary
-    const int head = min(end, begin + (int)((-reinterpret_cast<uintptr_t>(x + begin) & 15) / sizeof(T)));
-    const int vecs = (end - head) / VE, tail = head + vecs * VE;
     if ((int)threadIdx.x < head - begin) dx[begin + threadIdx.x] = from_f32<T>(grad(to_f32(x[begin + threadIdx.x])));
     if ((int)threadIdx.x < end - tail) dx[tail + threadIdx.x] = from_f32<T>(grad(to_f32(x[tail + threadIdx.x])));
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
     uint4* dv = reinterpret_cast<uint4*>(dx + head);
-    for (int v0 = threadIdx.x; v0 < vecs; v0 += kVecs * 256) {
-      uint4 w[kVecs];
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i)
-        if (v0 + i * 256 < vecs) w[i] = __ldcs(xv + v0 + i * 256);
+    for (int v0 = threadIdx.x;;) {
 #pragma unroll
       for (int i = 0; i < kVecs; ++i) {
-        if (v0 + i * 256 < vecs) {
+        if (v0 + i * NT < vecs) {
           float z[VE];
           unpack16<T>(w[i], z);
 #pragma unroll
           for (int k = 0; k < VE; ++k) z[k] = grad(z[k]);
-          dv[v0 + i * 256] = pack16<T>(z);
+          dv[v0 + i * NT] = pack16<T>(z);
         }
       }
+      v0 += kVecs * NT;
+      if (v0 >= vecs) break;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        if (v0 + i * NT < vecs) w[i] = __ldcs(xv + v0 + i * NT);
     }
   } else {
-    for (int j = begin + threadIdx.x; j < end; j += 256) dx[j] = from_f32<T>(grad(to_f32(x[j])));
+    for (int j = begin + threadIdx.x; j < end; j += NT) dx[j] = from_f32<T>(grad(to_f32(x[j])));
   }
   __syncthreads();
-  if ((int)threadIdx.x < n_fix && s != 0.f) {
+  if ((int)threadIdx.x < n_fix && !none) {
     const int j = s_idx[threadIdx.x];
     if (j >= begin && j < end) {
-      float g = 0.f;
-      for (int i = 0; i < n_fix; ++i) g += s_idx[i] == j ? s_g[i] : 0.f;
-      dx[j] = from_f32<T>(g + grad(to_f32(x[j])));
+      float own = 0.f, others = 0.f;
+      for (int i = 0; i < n_fix; ++i) (s_idx[i] == j ? own : others) += s_g[i];
+      // own - p own as own (1 - p), with 1 - p from the excess r: p may be nearly 1
+      const float d = below_max(to_f32(x[j]), m);
+      dx[j] = from_f32<T>(own * ((r - expm1f(d)) * inv) - exp_of(d) * inv * (others + e * ((d - log_s) + H)));
     }
   }
 }
@@ -531,8 +587,8 @@ int launch_fwd_nt(LpArgs& a, cudaStream_t st) {
 }
 
 // Threads a row: few for short rows and where many rows fill the GPU anyway (less waiting for one
-// another: 16384 x 32000 bf16 with 5 alternatives 224 us with 128, 274 us with 256; 20000 x 2000 fp16
-// 52 us with 64, 83 us with 128), many for few rows or long ones (64 x 32000 bf16: 7.6 us with 256, 8.2 us
+// another: 16384 x 32000 bf16 with 5 alternatives 229 us with 128, 266 us with 256; 20000 x 2000 fp16
+// 57 us with 64, 89 us with 128), many for few rows or long ones (64 x 32000 bf16: 7.6 us with 256, 8.2 us
 // with 128; 1500 x 150001 with 32 alternatives 213 us against 458 us).
 template <typename T>
 int launch_fwd(LpArgs& a, cudaStream_t st) {
@@ -542,19 +598,35 @@ int launch_fwd(LpArgs& a, cudaStream_t st) {
   return launch_fwd_nt<T, 256>(a, st);
 }
 
-template <typename T>
-int launch_bwd(LpBwdArgs& a, cudaStream_t st) {
-  constexpr int kChunk = 256 * 4 * 16 / sizeof(T);  // one round of every thread's vectors
-  a.chunks = (int)(((int64_t)a.V + kChunk - 1) / kChunk);
+template <typename T, int NT>
+int launch_bwd_nt(LpBwdArgs& a, cudaStream_t st) {
+  // four vectors a thread, twice where the CTAs are more than run at once: what a CTA prepares weighs half
+  // (16384 x 32000 bf16 321 us, with one round 336 us, both at 32 registers; one row of 32000 3.5 us with
+  // one round, 4.3 with two)
+  constexpr int64_t kRound = 64 * NT / (int64_t)sizeof(T);
+  int64_t chunk = kRound;
+  if (a.rows * ((a.V + kRound - 1) / kRound) > 1536 / NT * (int64_t)nfb_num_sms()) chunk *= 2;
+  a.chunks = (int)((a.V + chunk - 1) / chunk);
   // chunks of whole 16-byte pieces and of like size
   a.per = (int)((((int64_t)a.V + a.chunks - 1) / a.chunks + 7) / 8 * 8);
   if (a.rows * a.chunks > INT_MAX) return (int)cudaErrorInvalidValue;
   const bool vec = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.d_logits)) & 15) == 0 &&
                    (a.ld - a.V) * (int64_t)sizeof(T) % 16 == 0;
   const unsigned grid = (unsigned)(a.rows * a.chunks);
-  if (vec) logprobs_bwd_kernel<T, true><<<grid, 256, 0, st>>>(a);
-  else logprobs_bwd_kernel<T, false><<<grid, 256, 0, st>>>(a);
+  if (vec) logprobs_bwd_kernel<T, NT, true><<<grid, NT, 0, st>>>(a);
+  else logprobs_bwd_kernel<T, NT, false><<<grid, NT, 0, st>>>(a);
   return (int)cudaGetLastError();
+}
+
+// Threads a CTA: few for short rows, so that as many rows are under way as threads allow and fewer idle
+// (20000 x 2000 fp16 35 us with 64, 44 us with 128, 64 us with 256; 6000 x 8003 bf16 38 us with 128,
+// 42 us with 256); of no weight where a row has several chunks.
+template <typename T>
+int launch_bwd(LpBwdArgs& a, cudaStream_t st) {
+  const int64_t bytes = a.V * (int64_t)sizeof(T);
+  if (bytes <= 8192) return launch_bwd_nt<T, 64>(a, st);
+  if (bytes <= 16384) return launch_bwd_nt<T, 128>(a, st);
+  return launch_bwd_nt<T, 256>(a, st);
 }
 
 }  // namespace

@@ -245,9 +245,9 @@ NFB_EXPORT int nfb_paged_attn(int dtype, const void* q, const void* k_cache, con
                               const int64_t* dims, float scale, uint32_t* status, void* stream);
 
 /* ---- token log probabilities, entropy and top alternatives (logprobs.cu) ----------------- */
-/* stats (may be null) receives (max, sum of exp(z - max)) per row for the backward pass; targets may be null. A
- * target outside [0, V) other than ignore_index gives NaN and sets the status word (code 3).
- * top_k <= 32. */
+/* stats (may be null) receives (max, sum of exp(z - max) over all but one maximum) per row for the
+ * backward pass; targets may be null. A target outside [0, V) other than ignore_index gives NaN and
+ * sets the status word (code 3). top_k <= 32. */
 NFB_EXPORT int nfb_logprobs_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int64_t V,
                                 const int64_t* targets, int64_t ignore_index, int top_k, float* logprobs,
                                 float* entropy, float* stats, float* top_logprobs, int64_t* top_tokens,

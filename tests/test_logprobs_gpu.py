@@ -157,6 +157,34 @@ def test_masked_logits(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [3, 40, 2001, 32003, 150001])
+def test_rows_with_their_mass_on_one_token_keep_their_digits(dtype, V):
+    """log p = -log(1 + r) for a small r: the relative error is that of r (ts), not 2^-24 / r; so is that of the
+    gradient at the token, g r / (1 + r), and of the entropy (both parts positive)."""
+    g = _gen(V)
+    for M in (1, 5, 300):
+        x = (torch.randn(M, V, generator=g, device=DEV) * 2).to(dtype)
+        t = torch.randint(0, V, (M,), generator=g, device=DEV)
+        x[torch.arange(M, device=DEV), t] = (14 + 8 * torch.rand(M, generator=g, device=DEV)).to(dtype)
+        one, none = torch.ones(M, device=DEV), torch.zeros(M, device=DEV)
+        ref = _plain64(x, t, 0, -100, one, none, torch.zeros(M, 0, device=DEV))
+        lp64 = torch.log_softmax(x.double(), -1)
+        r64 = torch.where(torch.nn.functional.one_hot(t, V).bool(), torch.zeros_like(lp64), (x.double() - x.double().gather(1, t[:, None])).exp()).sum(-1)
+        leaf = x.clone().requires_grad_(True)
+        r = token_logprobs(leaf, t, top_k=1)
+        rel = ref["ts"] + 2.0 ** -21
+        want = -torch.log1p(r64)
+        assert ((r.logprobs.double() - want).abs() <= rel * want.abs()).all()
+        assert torch.equal(r.top_logprobs[:, 0], r.logprobs) and torch.equal(r.top_tokens[:, 0], t)
+        H = torch.log1p(r64) - ((lp64 - lp64.gather(1, t[:, None])).exp() * (x.double() - x.double().gather(1, t[:, None]))).sum(-1) / (1 + r64)
+        assert ((r.entropy.double() - H).abs() <= 2 * rel * H + 2.0 ** -120).all()
+        (dx,) = torch.autograd.grad(r.logprobs.sum(), leaf)
+        at = dx.gather(1, t[:, None])[:, 0].double()
+        tiny = {torch.float16: 2.0 ** -25}.get(dtype, 2.0 ** -126)
+        assert ((at - r64 / (1 + r64)).abs() <= (rel + torch.finfo(dtype).eps / 2) * r64 + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_nan_and_infinite_logits_stay_in_their_rows(dtype):
     for V in (64, 40000):
         x, t = _logits(5, V, dtype, seed=3)
