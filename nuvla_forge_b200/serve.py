@@ -124,17 +124,18 @@ class ReasoningDecoder:
         self.states = torch.zeros((B, self.n_prompt + N, model.cfg.t_dim), dtype=model.lm_head.dtype, device=dev)
         self.graph = None
         if graph and dev.type == "cuda":
-            side = torch.cuda.Stream(dev)
-            side.wait_stream(torch.cuda.current_stream(dev))
-            with torch.cuda.stream(side):
-                for _ in range(warmup):
-                    self._restart()
+            with torch.cuda.device(dev):  # the capture is of the current device's stream
+                side = torch.cuda.Stream(dev)
+                side.wait_stream(torch.cuda.current_stream(dev))
+                with torch.cuda.stream(side):
+                    for _ in range(max(1, warmup)):  # (the status words are made outside of the capture)
+                        self._restart()
+                        self._step()
+                torch.cuda.current_stream(dev).wait_stream(side)
+                self._restart()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
                     self._step()
-            torch.cuda.current_stream(dev).wait_stream(side)
-            self._restart()
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
-                self._step()
             self.graph = g
 
     def _restart(self) -> None:
