@@ -143,7 +143,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
         return TokenLogprobs(*r)
     lp, h, top, ids = r
     return TokenLogprobs(None if lp is None else lp.view(lead), h.view(lead),
-                         None if top is None else top.view(*lead, top_k), None if ids is None else ids.view(*lead, top_k))
+                         None if top is None else top.view(*lead, top_k),
+                         None if ids is None else ids.view(*lead, top_k))
 
 
 __all__ = ["MAX_TOP_K", "TokenLogprobs", "check_status", "token_logprobs"]
