@@ -19,6 +19,7 @@ from .. import _native as nat
 from .reference import token_logprobs_ref
 
 MAX_TOP_K = 32
+_BAD_TARGET = 3 << 24 | 1  # the kernel's status: code 3 (bad argument), site 1
 
 _status: dict[int, torch.Tensor] = {}
 
@@ -94,6 +95,17 @@ class _TokenLogprobs(torch.autograd.Function):
         return dx, None, None, None
 
 
+def _reference_on_device(x, targets, top_k, ignore_index, word):
+    """The reference without its index check: a target outside the vocabulary (torch's gather would abort the
+    process's GPU context) gives NaN, no gradient, and the status that the kernel sets in ``word``."""
+    if targets is None:
+        return token_logprobs_ref(x, None, top_k, ignore_index)
+    bad = (targets != ignore_index) & ((targets < 0) | (targets >= x.shape[1]))
+    given, *rest = token_logprobs_ref(x, targets.masked_fill(bad, ignore_index), top_k, ignore_index)
+    word.copy_(torch.where(bad.any(), torch.full_like(word, _BAD_TARGET), word))
+    return given.masked_fill(bad, float("nan")), *rest
+
+
 # gradients of the gradient raise instead of being silently zero
 _first_order = once_differentiable(_TokenLogprobs._gradient)
 
@@ -130,7 +142,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     x = logits if flat else logits.reshape(-1, V)
     t = targets if flat or targets is None else targets.reshape(-1)
     if force_reference or not (nat.HAS_NATIVE and x.is_cuda and x.dtype in nat.DT):
-        r = token_logprobs_ref(x, t, top_k, ignore_index)
+        r = _reference_on_device(x, t, top_k, ignore_index, _status_word(x.device)) if x.is_cuda else \
+            token_logprobs_ref(x, t, top_k, ignore_index)
     else:
         if x.stride(1) != 1 and V > 1:
             x = x.contiguous()
