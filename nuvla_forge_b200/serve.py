@@ -25,6 +25,7 @@ The reference has no inference path beyond ``TrajectoryDiT.sample``
 
 from __future__ import annotations
 
+import threading
 from typing import NamedTuple
 
 import torch
@@ -94,7 +95,9 @@ class ReasoningDecoder:
 
     Built for a batch size, ``prompt_len`` instruction tokens and ``max_new`` answer tokens (at most
     the model's text positions together). ``stop_token`` ends a sequence: its later tokens repeat it,
-    are not stored and score 0. The reference has no decoding path.
+    are not stored and score 0. A decoder works on one answer at a time: calls from several threads
+    or streams wait for one another (build a decoder for each to have them at once). The reference has
+    no decoding path.
     """
 
     def __init__(self, model: NuVLA, batch_size: int, prompt_len: int, max_new: int | None = None, top_k: int = 5,
@@ -123,6 +126,8 @@ class ReasoningDecoder:
         self.lengths = torch.zeros(B, dtype=torch.int64, device=dev)
         self.states = torch.zeros((B, self.n_prompt + N, model.cfg.t_dim), dtype=model.lm_head.dtype, device=dev)
         self.graph = None
+        self._turn = threading.Lock()
+        self._done: torch.cuda.Event | None = None   # the last use of the buffers above, on any stream
         if graph and dev.type == "cuda":
             with torch.cuda.device(dev):  # the capture is of the current device's stream
                 side = torch.cuda.Stream(dev)
@@ -137,6 +142,9 @@ class ReasoningDecoder:
                 with torch.cuda.graph(g):
                     self._step()
             self.graph = g
+        if dev.type == "cuda":
+            self._done = torch.cuda.Event()
+            self._done.record(torch.cuda.current_stream(dev))
 
     def _restart(self) -> None:
         self.index.zero_()
@@ -179,6 +187,20 @@ class ReasoningDecoder:
         if text_tokens.shape != (self.batch_size, self.prompt_len):
             raise ValueError(f"decoder was built for instructions {(self.batch_size, self.prompt_len)}, got "
                              f"{tuple(text_tokens.shape)}")
+        with self._turn:
+            if self._done is None:
+                return self._answer(images, text_tokens)
+            stream = torch.cuda.current_stream(self.token.device)
+            captured = torch.cuda.is_current_stream_capturing()  # (ordered by whoever replays it)
+            if not captured:
+                stream.wait_event(self._done)
+            try:
+                return self._answer(images, text_tokens)
+            finally:
+                if not captured:
+                    self._done.record(stream)
+
+    def _answer(self, images: torch.Tensor, text_tokens: torch.Tensor) -> Answer:
         h = self.model.read_prompt(images, text_tokens, self.cache)
         if h.shape[1] != self.n_prompt:
             raise ValueError(f"decoder was built for {self.n_prompt} prompt states, got {h.shape[1]}")

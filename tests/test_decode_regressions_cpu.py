@@ -1,9 +1,27 @@
 """Cached decoding and scores on the CPU: calls that once went wrong."""
 
+import threading
+import time
+
 import pytest
 import torch
 
+from nuvla_forge_b200.models import NuVLA, NuVLAConfig
 from nuvla_forge_b200.ops import logprobs as lp
+from nuvla_forge_b200.serve import ReasoningDecoder
+
+
+def _model(**over):
+    torch.manual_seed(0)
+    cfg = NuVLAConfig.preset("tiny", image_size=32, n_views=2, n_frames=1, vision_dim=64, vision_depth=1, vision_heads=2,
+                             text_dim=64, text_depth=2, text_heads=4, text_kv_heads=2, text_ffn=128, dit_dim=64,
+                             dit_depth=1, dit_heads=2, vocab_size=120, n_instruction=5, n_reasoning=9, **over)
+    model = NuVLA(cfg)
+    with torch.no_grad():
+        model.lm_head.mul_(20.0)                      # clear winners among the tokens
+    images = torch.randint(0, 256, (3, 2, 32, 32, 3), dtype=torch.uint8)
+    text = torch.randint(0, 120, (3, 5))
+    return model, images, text
 
 
 def test_reference_scores_of_device_tensors_never_index_with_a_bad_target():
@@ -26,3 +44,34 @@ def test_reference_scores_of_device_tensors_never_index_with_a_bad_target():
     assert lp._reference_on_device(x, None, 0, -100, word)[0] is None
     with pytest.raises(RuntimeError):
         lp.token_logprobs(x, torch.tensor([3, -100, 9, 8]))       # a CPU tensor: torch's own check
+
+
+def test_two_threads_share_a_decoder_one_call_at_a_time(monkeypatch):
+    """Calls in each other's buffers count positions past their end (on a GPU a device assert)."""
+    model, images, text = _model()
+    texts = [text, torch.randint(0, 120, (3, 5))]
+    want = [ReasoningDecoder(model, 3, 5, max_new=4)(images, t) for t in texts]
+    dec = ReasoningDecoder(model, 3, 5, max_new=4)
+    busy, most, got, read = [0], [0], [None, None], model.read_prompt
+
+    def slow(*args):
+        busy[0] += 1
+        most[0] = max(most[0], busy[0])
+        time.sleep(0.2)
+        h = read(*args)
+        busy[0] -= 1
+        return h
+
+    monkeypatch.setattr(model, "read_prompt", slow)
+
+    def call(i):
+        got[i] = dec(images, texts[i])
+
+    threads = [threading.Thread(target=call, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert most[0] == 1
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -3,10 +3,24 @@
 import pytest
 import torch
 
+from nuvla_forge_b200.models import NuVLA, NuVLAConfig
 from nuvla_forge_b200.ops import logprobs as lp
+from nuvla_forge_b200.ops import paged
+from nuvla_forge_b200.serve import ReasoningDecoder
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+
+def _model(dtype, **over):
+    torch.manual_seed(0)
+    cfg = NuVLAConfig.preset("tiny", vocab_size=1000, n_instruction=8, n_reasoning=40, **over)
+    model = NuVLA(cfg)
+    with torch.no_grad():
+        model.lm_head.mul_(10.0)
+    model = model.to(DEV, dtype)
+    images = torch.randint(0, 256, (4, cfg.n_images, 128, 128, 3), dtype=torch.uint8, device=DEV)
+    return model, images, torch.randint(0, 1000, (4, 8), device=DEV)
 
 
 def test_bad_targets_of_64_bit_logits_are_reported():
@@ -19,3 +33,23 @@ def test_bad_targets_of_64_bit_logits_are_reported():
         with pytest.raises(RuntimeError, match="outside the vocabulary"):
             lp.check_status()
     lp.check_status()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_two_streams_share_a_decoder_one_call_at_a_time(graph):
+    model, images, text = _model(torch.bfloat16)
+    texts = [text] + [torch.randint(0, 1000, (4, 8), device=DEV) for _ in range(3)]
+    dec = ReasoningDecoder(model, 4, 8, max_new=12, graph=graph)
+    want = [dec(images, t) for t in texts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i, t in enumerate(texts):
+        with torch.cuda.stream(streams[i % 2]):
+            if i == 0:
+                torch.cuda._sleep(20_000_000)         # the others are enqueued before the first one runs
+            got.append(dec(images, t))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    paged.check_status()
