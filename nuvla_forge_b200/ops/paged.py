@@ -96,8 +96,9 @@ def _native(t: torch.Tensor) -> bool:
 
 
 def _rows_ok(*tensors) -> bool:
-    """Whether the kernels read the tensors as they are: unit inner stride."""
-    return all(t is None or t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 for t in tensors)
+    """Whether the kernels read the tensors as they are: unit inner stride, or (``contiguous`` returns an empty
+    tensor as it is) nothing to read."""
+    return all(t is None or t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 or t.numel() == 0 for t in tensors)
 
 
 def _append_plan(key, k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved) -> tuple:

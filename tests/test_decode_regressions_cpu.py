@@ -8,6 +8,7 @@ import torch
 
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig
 from nuvla_forge_b200.ops import logprobs as lp
+from nuvla_forge_b200.ops import paged
 from nuvla_forge_b200.serve import ReasoningDecoder
 
 
@@ -75,3 +76,10 @@ def test_two_threads_share_a_decoder_one_call_at_a_time(monkeypatch):
     assert most[0] == 1
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_empty_tensors_of_any_stride_are_read_as_they_are():
+    """``contiguous`` leaves an empty tensor's strides, so asking it for unit ones never ended."""
+    for t in (torch.zeros(0, 1, 64, 8).transpose(2, 3), torch.zeros(2, 8, 0, 4).permute(0, 2, 3, 1),
+              torch.zeros(3, 0, dtype=torch.int32).T, torch.zeros(4, 6)[:, ::2], torch.zeros(4, 6).T[:, 1:3]):
+        assert paged._rows_ok(paged._inner(t))

@@ -53,3 +53,16 @@ def test_two_streams_share_a_decoder_one_call_at_a_time(graph):
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
     paged.check_status()
+
+
+def test_empty_calls_of_any_stride():
+    kc, vc = (torch.zeros(2, 16, 2, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    e = torch.zeros(0, dtype=torch.int32, device=DEV)
+    q = torch.zeros(0, 1, 64, 4, device=DEV, dtype=torch.bfloat16).transpose(2, 3)
+    assert paged.paged_attention(q, kc, vc, e.view(0, 1), e).shape == (0, 1, 4, 64)
+    k = torch.zeros(0, 3, 64, 2, device=DEV, dtype=torch.bfloat16).transpose(2, 3)
+    assert paged.append_kv(k, k, kc, vc, e.view(0, 1), e, q=k).shape == (0, 3, 2, 64)
+    k = torch.zeros(2, 0, 64, 2, device=DEV, dtype=torch.bfloat16).transpose(2, 3)
+    n = torch.zeros(2, dtype=torch.int32, device=DEV)
+    assert paged.append_kv(k, k, kc, vc, n.view(2, 1), n, q=k).shape == (2, 0, 2, 64)
+    paged.check_status()
