@@ -226,11 +226,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return paged_attention(_inner(q), k_cache, v_cache, _inner(page_table), _inner(lengths), sc)
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    # the caching allocator's memory, new for each call: calls on other streams and in other graphs have theirs
-    ws = torch.empty(n_ws, dtype=torch.float32, device=dev).data_ptr() if n_ws else None
+    # the caching allocator's memory, new for each call and held until its kernels are launched: calls on other
+    # streams, in other threads and in other graphs have theirs
+    ws = torch.empty(n_ws, dtype=torch.float32, device=dev) if n_ws else None
     with nat.on_device(dev):
         nat.call("nfb_paged_attn", nat.DT[q.dtype], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                 page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), ws, dims, sc,
+                 page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), nat.ptr(ws), dims, sc,
                  _status_word(dev).data_ptr(), nat.stream(dev))
     return out
 

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from nuvla_forge_b200 import _native as nat
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig
 from nuvla_forge_b200.ops import logprobs as lp
 from nuvla_forge_b200.ops import paged
@@ -66,3 +67,25 @@ def test_empty_calls_of_any_stride():
     n = torch.zeros(2, dtype=torch.int32, device=DEV)
     assert paged.append_kv(k, k, kc, vc, n.view(2, 1), n, q=k).shape == (2, 0, 2, 64)
     paged.check_status()
+
+
+def test_workspace_is_held_until_the_kernels_are_launched(monkeypatch):
+    """Another thread that allocates on the same stream in the meantime must not be handed the call's workspace."""
+    kc, vc = (torch.randn(100, 16, 4, 64, device=DEV).to(torch.bfloat16) for _ in range(2))
+    table = torch.arange(100, dtype=torch.int32, device=DEV)[None]
+    lengths = torch.tensor([1600], dtype=torch.int32, device=DEV)
+    q = torch.randn(1, 1, 8, 64, device=DEV).to(torch.bfloat16)
+    want = paged.paged_attention(q, kc, vc, table, lengths)
+    call, seen = nat.call, []
+
+    def between(name, *args):
+        ws = args[7]
+        assert name == "nfb_paged_attn" and ws is not None
+        n = int(nat.lib().nfb_paged_attn_ws(1, 8, 4, 64, 1600))
+        other = [torch.empty(n, device=DEV) for _ in range(4)]       # of the workspace's size
+        seen.append(all(not t.data_ptr() <= ws < t.data_ptr() + 4 * n for t in other))
+        return call(name, *args)
+
+    monkeypatch.setattr(nat, "call", between)
+    got = paged.paged_attention(q, kc, vc, table, lengths)
+    assert seen == [True] and torch.equal(got, want)
