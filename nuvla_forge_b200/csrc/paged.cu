@@ -526,13 +526,19 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attn_plain_kernel(const AttnA
 // tail and the join; one sequence of 131001 tokens 89 us (6.05 TB/s).
 //
 // The weights p = exp(z - m) would lose 8 bits (bf16) as an operand, so they go in as two: hi, p
-// rounded a little low so that p - hi > 0, and the rest; one step is two products, 2^-16 of p is left
-// (fp16: 2^-20), and an infinite value stays infinite because both parts are positive. Sums of
-// weights use the fp32 values. The running maximum moves only when a score passes it by more than
-// 2^8: the sums have the room, and the rescaling, with its exchange between lanes, becomes rare.
+// rounded a little low so that p - hi > 0, and the rest; one step is two products, 2^-16 of p is left,
+// and an infinite value stays infinite because both parts are positive. Sums of weights use the fp32
+// values. The running maximum moves only when a score passes it by more than kRoom (a factor of 2^8):
+// the sums have the room, and the rescaling, with its exchange between lanes, becomes rare.
+//
+// fp16 has the digits (2^-20 of p) but not the range: its parts of a p below 2^-4 would be subnormal, and
+// a p below 2^-25 gone from the values while it stays in the sum. So they are 2^14 p, as large as fp16
+// holds with a factor of 2 left for the lazy maximum (p <= 2), and the output is scaled back. Left of p
+// are 2^-20 p or 2^-39, whichever is more: the 2^17 smallest weights of a long cache add up to 2^-22.
+// (An infinite value stays infinite down to p = 2^-28; below, the second part may be 0.)
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
-  static constexpr float kLow = 1.f - 0x1p-8f;
+  static constexpr float kLow = 1.f - 0x1p-8f, kScale = 1.f, kRoom = 8.f;
   static __device__ __forceinline__ void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -548,7 +554,7 @@ template <> struct Mma<__nv_bfloat16> {
   }
 };
 template <> struct Mma<__half> {
-  static constexpr float kLow = 1.f - 0x1p-10f;
+  static constexpr float kLow = 1.f - 0x1p-10f, kScale = 0x1p14f, kRoom = 1.f;
   static __device__ __forceinline__ void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -805,7 +811,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, attn_ctas(D, NG)) attn_mma_ke
           for (int i = 0; i < 4; ++i) z[i] = mask >> (r + 8 * (i >> 1)) & 1 ? z[i] : -INFINITY;
         }
         float mx[2] = {fmaxf(z[0], z[2]), fmaxf(z[1], z[3])};
-        if (__any_sync(0xffffffffu, mx[0] > m[g][0] + 8.f || mx[1] > m[g][1] + 8.f)) {
+        if (__any_sync(0xffffffffu, mx[0] > m[g][0] + Mma<T>::kRoom || mx[1] > m[g][1] + Mma<T>::kRoom)) {
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -828,10 +834,11 @@ __global__ void __launch_bounds__(32 * kAttnWarps, attn_ctas(D, NG)) attn_mma_ke
         l[g][1] += e[1] + e[3];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t x = Mma<T>::pack(e[2 * h] * Mma<T>::kLow, e[2 * h + 1] * Mma<T>::kLow);
+          constexpr float kScale = Mma<T>::kScale, kHi = Mma<T>::kLow * kScale;
+          const uint32_t x = Mma<T>::pack(e[2 * h] * kHi, e[2 * h + 1] * kHi);
           const float2 f = Mma<T>::unpack(x);
           hi[g][h] = transpose8x8(x);
-          lo[g][h] = transpose8x8(Mma<T>::pack(e[2 * h] - f.x, e[2 * h + 1] - f.y));
+          lo[g][h] = transpose8x8(Mma<T>::pack(fmaf(e[2 * h], kScale, -f.x), fmaf(e[2 * h + 1], kScale, -f.y)));
         }
       }
 #pragma unroll
@@ -868,8 +875,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps, attn_ctas(D, NG)) attn_mma_ke
           float* so = s_o + (warp * 4 + 2 * (j & 1) + n) * kPitchO + r;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
-            so[16 * t] = o[h4 / 2][t][n];
-            so[16 * t + 8] = o[h4 / 2][t][n + 2];
+            so[16 * t] = o[h4 / 2][t][n] * (1.f / Mma<T>::kScale);
+            so[16 * t + 8] = o[h4 / 2][t][n + 2] * (1.f / Mma<T>::kScale);
           }
         }
       }

@@ -89,3 +89,31 @@ def test_workspace_is_held_until_the_kernels_are_launched(monkeypatch):
     monkeypatch.setattr(nat, "call", between)
     got = paged.paged_attention(q, kc, vc, table, lengths)
     assert seen == [True] and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nats", [10, 14, 18])
+@pytest.mark.parametrize("B,hk,d,L", [(1, 1, 64, 768), (2, 4, 96, 700), (300, 8, 128, 8192)])
+def test_a_tail_of_small_weights_keeps_its_share(dtype, nats, B, hk, d, L):
+    """Four tokens with values of 0 (one for each warp) hold nearly all the mass; the output is what the tail
+    gives. p = exp(-nats), at least 2^-26: relative to the output, a weight as two 16-bit parts is off by 2^-16
+    (bf16) or 2^-20 + 2^-39 / p <= 2^-13 + 2^-20 (fp16), its exponential by 2^-22 and the score's three roundings
+    by 3 * 18 * 2^-24 < 2^-18, the sums by 2^-23 for each of the L / 16 + 64 steps. The output is rounded once."""
+    ps = 16
+    pages = -(-L // ps)
+    g = torch.Generator(DEV).manual_seed(nats + L)
+    kc = torch.zeros(pages, ps, hk, d, device=DEV, dtype=dtype)
+    kc[..., 0] = -nats                                # scores: exact, 0 for the four and -nats for the tail
+    vc = (1 + torch.rand(pages, ps, hk, d, generator=g, device=DEV)).to(dtype)
+    kc[:4, 5], vc[:4, 5] = 0, 0
+    q = torch.zeros(B, 1, hk, d, device=DEV, dtype=dtype)
+    q[..., 0] = 1
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).expand(B, pages)
+    lengths = torch.full((B,), L, dtype=torch.int32, device=DEV)
+    out = paged.paged_attention(q, kc, vc, table, lengths, scale=1.0)
+    z = kc.flatten(0, 1)[:L, :, 0].double()
+    want = torch.einsum("lh,lhd->hd", torch.softmax(z, 0), vc.flatten(0, 1)[:L].double())
+    rel = 2.0 ** -13 + 2.0 ** -16 + 2.0 ** -18 + 2.0 ** -20 + (L / 16 + 64) * 2.0 ** -23 + torch.finfo(dtype).eps / 2
+    # (fp16: outputs below 2^-14 are rounded to a multiple of 2^-24)
+    assert ((out[:, 0].double() - want).abs() <= rel * want + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
+    paged.check_status()
