@@ -21,6 +21,7 @@ import os
 from ctypes import c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
 
 import torch
+from torch.autograd import forward_ad as fwd_ad
 
 from ._build import build, lib_path
 
@@ -223,6 +224,11 @@ def stream(device: torch.device | None = None) -> int:
 def int64s(*values: int):
     """A host array of int64 for entry points that take their sizes and strides as one array."""
     return (c_int64 * len(values))(*values)
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a forward-mode derivative, which a kernel called past autograd would drop."""
+    return fwd_ad._current_level >= 0 and any(t is not None and fwd_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _NO_GUARD = contextlib.nullcontext()

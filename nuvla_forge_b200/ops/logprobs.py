@@ -145,6 +145,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
         r = _reference_on_device(x, t, top_k, ignore_index, _status_word(x.device)) if x.is_cuda else \
             token_logprobs_ref(x, t, top_k, ignore_index)
     else:
+        if nat.has_tangent(x):
+            raise RuntimeError("token_logprobs has no forward-mode derivative on a GPU: use force_reference")
         if x.stride(1) != 1 and V > 1:
             x = x.contiguous()
         t = None if t is None else t.contiguous()

@@ -14,7 +14,7 @@ streams can run them at once on caches of their own.
 
 A position or page id out of range cannot be refused without reading it back: the kernels skip the
 token and set a status word that ``check_status`` (and the trainer's health monitor) raises on. On
-the CPU the reference raises IndexError. Neither op has a backward pass.
+the CPU the reference raises IndexError. Neither op has a derivative.
 
 The reference project has no decoding path.
 """
@@ -162,6 +162,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
             or (q is not None and q.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("append_kv has no backward pass: call it under torch.no_grad()")
+    if nat.has_tangent(k, v, k_cache, v_cache, q, cos, sin):
+        raise RuntimeError("append_kv has no forward-mode derivative")
     if force_reference or not native:
         out = append_kv_ref(k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
         return out.clone() if out is q and q is not None else out
@@ -219,6 +221,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     native, dims, n_ws, default = plan
     if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("paged_attention has no backward pass: call it under torch.no_grad()")
+    if nat.has_tangent(q, k_cache, v_cache):
+        raise RuntimeError("paged_attention has no forward-mode derivative")
     sc = default if scale is None else float(scale)
     if force_reference or not native:
         return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, sc)

@@ -5,6 +5,7 @@ import time
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig
 from nuvla_forge_b200.ops import logprobs as lp
@@ -83,3 +84,24 @@ def test_empty_tensors_of_any_stride_are_read_as_they_are():
     for t in (torch.zeros(0, 1, 64, 8).transpose(2, 3), torch.zeros(2, 8, 0, 4).permute(0, 2, 3, 1),
               torch.zeros(3, 0, dtype=torch.int32).T, torch.zeros(4, 6)[:, ::2], torch.zeros(4, 6).T[:, 1:3]):
         assert paged._rows_ok(paged._inner(t))
+
+
+def test_forward_mode_derivatives_are_right_or_refused():
+    torch.manual_seed(0)
+    x, d = torch.randn(3, 9, dtype=torch.float64), torch.randn(3, 9, dtype=torch.float64)
+    t = torch.tensor([1, 8, 0])
+    k, kc = torch.randn(2, 1, 2, 8), torch.randn(4, 4, 2, 8)
+    table, n = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32), torch.tensor([3, 4], dtype=torch.int32)
+    with forward_ad.dual_level():
+        r = lp.token_logprobs(forward_ad.make_dual(x, d), t)
+        logp = torch.log_softmax(x, -1)
+        want = d.gather(1, t[:, None])[:, 0] - (logp.exp() * d).sum(-1)
+        assert (forward_ad.unpack_dual(r.logprobs).tangent - want).abs().max() < 1e-12
+        dual = forward_ad.make_dual(k, torch.ones_like(k))
+        for bad in (dict(k=dual, v=k), dict(k=k, v=dual), dict(k=k, v=k, q=dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                paged.append_kv(**bad, k_cache=kc.clone(), v_cache=kc.clone(), page_table=table, lengths=n)
+        for q, c in ((dual, kc), (k, forward_ad.make_dual(kc, kc))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                paged.paged_attention(q, c, kc, table, n)
+        paged.paged_attention(k, kc, kc, table, n)    # nothing dual among the arguments

@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from nuvla_forge_b200 import _native as nat
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig
@@ -117,3 +118,23 @@ def test_a_tail_of_small_weights_keeps_its_share(dtype, nats, B, hk, d, L):
     # (fp16: outputs below 2^-14 are rounded to a multiple of 2^-24)
     assert ((out[:, 0].double() - want).abs() <= rel * want + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
     paged.check_status()
+
+
+def test_forward_mode_derivatives_are_refused():
+    x, d = (torch.randn(3, 90, device=DEV) for _ in range(2))
+    kc = torch.randn(4, 16, 2, 64, device=DEV)
+    k, n = torch.randn(2, 1, 2, 64, device=DEV), torch.tensor([3, 4], dtype=torch.int32, device=DEV)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, d)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            lp.token_logprobs(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+            lp.token_logprobs(dual)
+        assert forward_ad.unpack_dual(lp.token_logprobs(dual, force_reference=True).entropy).tangent is not None
+        dk = forward_ad.make_dual(k, k)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged.paged_attention(dk, kc, kc, n.view(2, 1), n)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            paged.append_kv(dk, k, kc, kc.clone(), n.view(2, 1), n)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda z: lp.token_logprobs(z).entropy, (x,), (d,))
