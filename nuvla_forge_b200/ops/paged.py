@@ -160,7 +160,8 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         plan = _append_plan(key, k, v, k_cache, v_cache, page_table, lengths, counts, q, cos, sin, interleaved)
     native, dims = plan
     if (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
-            or (q is not None and q.requires_grad)) and torch.is_grad_enabled():
+            or (q is not None and q.requires_grad)
+            or (cos is not None and (cos.requires_grad or sin.requires_grad))) and torch.is_grad_enabled():
         raise RuntimeError("append_kv has no backward pass: call it under torch.no_grad()")
     if nat.has_tangent(k, v, k_cache, v_cache, q, cos, sin):
         raise RuntimeError("append_kv has no forward-mode derivative")

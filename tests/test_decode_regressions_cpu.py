@@ -105,3 +105,14 @@ def test_forward_mode_derivatives_are_right_or_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 paged.paged_attention(q, c, kc, table, n)
         paged.paged_attention(k, kc, kc, table, n)    # nothing dual among the arguments
+
+
+def test_append_refuses_angles_that_require_a_gradient():
+    k, kc = torch.randn(2, 1, 2, 8), torch.randn(4, 4, 2, 8)
+    table, n = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32), torch.tensor([3, 4], dtype=torch.int32)
+    one, learned = torch.ones(8, 4), torch.ones(8, 4, requires_grad=True)
+    for cos, sin in ((learned, one), (one, learned)):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            paged.append_kv(k, k, kc, kc.clone(), table, n, cos=cos, sin=sin)
+        with torch.no_grad():
+            paged.append_kv(k, k, kc, kc.clone(), table, n, cos=cos, sin=sin)
