@@ -17,6 +17,7 @@ the next token.
     decoder = ReasoningDecoder(model, batch_size=8, prompt_len=64, max_new=256)
     answer = decoder(images, text_tokens)   # tokens, log probabilities, entropy, alternatives, states
     waypoints = planner(answer.states)      # the DiT attends to the answer's states too
+    waypoints = model.dit.sample(answer.context(b))   # or to one answer's, cut behind its stop token
 
 On CPU (or with ``graph=False``) both run the same code eagerly.
 The reference has no inference path beyond ``TrajectoryDiT.sample``
@@ -87,15 +88,22 @@ class Answer(NamedTuple):
     top_tokens: torch.Tensor     # [B, max_new, top_k] int64
     top_logprobs: torch.Tensor   # [B, max_new, top_k] fp32
     lengths: torch.Tensor        # [B] int64, tokens up to and with the stop token
-    states: torch.Tensor         # [B, prompt states + max_new, D], for the DiT's cross-attention
+    states: torch.Tensor         # [B, prompt states + max_new, D], for the DiT's cross-attention: those of
+                                 # ``model.context`` over instruction and ``tokens``, repeated stop tokens too
+
+    def context(self, b: int) -> torch.Tensor:
+        """States [1, n, D] of sequence ``b`` up to and with its stop token (waits for its length). The DiT attends to
+        every state that it is given, so a plan from these does not depend on ``max_new``, one from ``states`` does."""
+        n = self.states.shape[1] - self.tokens.shape[1] + int(self.lengths[b])
+        return self.states[b:b + 1, :n]
 
 
 class ReasoningDecoder:
     """Greedy answers of the reasoning head over a paged key-value cache (causal backbone layout).
 
     Built for a batch size, ``prompt_len`` instruction tokens and ``max_new`` answer tokens (at most
-    the model's text positions together). ``stop_token`` ends a sequence: its later tokens repeat it,
-    are not stored and score 0. A decoder works on one answer at a time: calls from several threads
+    the model's text positions together). ``stop_token`` ends a sequence: its later tokens repeat it and
+    score 0 (they are read like others, so that ``states`` are those of the returned tokens). A decoder works on one answer at a time: calls from several threads
     or streams wait for one another (build a decoder for each to have them at once). The reference has
     no decoding path.
     """
@@ -173,11 +181,8 @@ class ReasoningDecoder:
     def _step(self) -> None:
         """Read the token that was chosen last, choose the next one."""
         if self.stop_token is not None:
-            counts = self.live.clone()                            # the stop token itself is still read
             self.live.mul_((self.token != self.stop_token).to(torch.int32))
-        else:
-            counts = None
-        h = self.model.read_token(self.token, self.index + self.prompt_len, self.cache, counts)
+        h = self.model.read_token(self.token, self.index + self.prompt_len, self.cache)
         self.states.index_copy_(1, self.index + self.n_prompt, h)
         self.index.add_(1)
         self._choose(h[:, 0], self.index)

@@ -13,6 +13,11 @@ from nuvla_forge_b200.ops import paged
 from nuvla_forge_b200.serve import ReasoningDecoder
 
 
+# two fp32 evaluations of one small network (width 64, depth 2): a few hundred roundings of 2^-24 of
+# values below 30
+TOL = 300 * 30 * 2.0 ** -24
+
+
 def _model(**over):
     torch.manual_seed(0)
     cfg = NuVLAConfig.preset("tiny", image_size=32, n_views=2, n_frames=1, vision_dim=64, vision_depth=1, vision_heads=2,
@@ -116,3 +121,21 @@ def test_append_refuses_angles_that_require_a_gradient():
             paged.append_kv(k, k, kc, kc.clone(), table, n, cos=cos, sin=sin)
         with torch.no_grad():
             paged.append_kv(k, k, kc, kc.clone(), table, n, cos=cos, sin=sin)
+
+
+def test_states_behind_a_stop_token_are_those_of_the_returned_tokens():
+    model, images, text = _model()
+    free = ReasoningDecoder(model, 3, 5, max_new=7)(images, text)
+    stop = int(free.tokens[1, 2])
+    z0 = torch.randn(1, model.cfg.horizon, model.cfg.traj_dim)
+    plans = []
+    for max_new in (7, 9):
+        a = ReasoningDecoder(model, 3, 5, max_new=max_new, stop_token=stop)(images, text)
+        assert int(a.lengths[1]) <= 3
+        with torch.no_grad():
+            whole = model.context(images, torch.cat([text, a.tokens], 1))
+            assert (a.states - whole).abs().max() < TOL
+            one = model.context(images[1:2], torch.cat([text[1:2], a.tokens[1:2, : int(a.lengths[1])]], 1))
+            assert a.context(1).shape == one.shape and (a.context(1) - one).abs().max() < TOL
+            plans.append(model.dit.sample(a.context(1), steps=2, z0=z0))
+    assert (plans[0] - plans[1]).abs().max() < TOL
