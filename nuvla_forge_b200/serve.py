@@ -83,9 +83,9 @@ class GraphedPlanner:
 
 class Answer(NamedTuple):
     tokens: torch.Tensor         # [B, max_new] int64
-    logprobs: torch.Tensor       # [B, max_new] fp32, of the tokens (0 behind a stop token)
+    logprobs: torch.Tensor       # [B, max_new] fp32, of the tokens (behind a stop token all scores are 0)
     entropy: torch.Tensor        # [B, max_new] fp32, of each token's distribution
-    top_tokens: torch.Tensor     # [B, max_new, top_k] int64
+    top_tokens: torch.Tensor     # [B, max_new, top_k] int64 (behind a stop token that token)
     top_logprobs: torch.Tensor   # [B, max_new, top_k] fp32
     lengths: torch.Tensor        # [B] int64, tokens up to and with the stop token
     states: torch.Tensor         # [B, prompt states + max_new, D], for the DiT's cross-attention: those of
@@ -165,17 +165,18 @@ class ReasoningDecoder:
     def _choose(self, h: torch.Tensor, at: torch.Tensor) -> None:
         """The most likely next token of states h [B, D], written with its scores to column ``at`` [1]."""
         r = token_logprobs(self.model.text_logits(h), top_k=self.top_k, force_reference=not self.model.cfg.fused)
-        on = self.live.bool()
-        token = r.top_tokens[:, 0]
+        top, scores, entropy = r.top_tokens, r.top_logprobs, r.entropy
         if self.stop_token is not None:
-            token = torch.where(on, token, torch.full_like(token, self.stop_token))
-        self.token.copy_(token)
+            off = self.live == 0
+            top = top.masked_fill(off[:, None], self.stop_token)
+            scores, entropy = scores.masked_fill(off[:, None], 0.0), entropy.masked_fill(off, 0.0)
+        self.token.copy_(top[:, 0])
         self.lengths.add_(self.live)
-        self.tokens.index_copy_(1, at, token[:, None])
-        self.logprobs.index_copy_(1, at, (r.top_logprobs[:, 0] * on)[:, None])
-        self.entropy.index_copy_(1, at, (r.entropy * on)[:, None])
-        self.top_tokens.index_copy_(1, at, r.top_tokens[:, None])
-        self.top_logprobs.index_copy_(1, at, r.top_logprobs[:, None])
+        self.tokens.index_copy_(1, at, top[:, :1])
+        self.logprobs.index_copy_(1, at, scores[:, :1])
+        self.entropy.index_copy_(1, at, entropy[:, None])
+        self.top_tokens.index_copy_(1, at, top[:, None])
+        self.top_logprobs.index_copy_(1, at, scores[:, None])
 
     @torch.no_grad()
     def _step(self) -> None:

@@ -139,3 +139,22 @@ def test_states_behind_a_stop_token_are_those_of_the_returned_tokens():
             assert a.context(1).shape == one.shape and (a.context(1) - one).abs().max() < TOL
             plans.append(model.dit.sample(a.context(1), steps=2, z0=z0))
     assert (plans[0] - plans[1]).abs().max() < TOL
+
+
+def test_every_score_behind_a_stop_token_is_zero():
+    model, images, text = _model()
+    free = ReasoningDecoder(model, 3, 5, max_new=7, top_k=3)(images, text)
+    stop = int(free.tokens[1, 2])
+    a = ReasoningDecoder(model, 3, 5, max_new=7, top_k=3, stop_token=stop)(images, text)
+    n = int(a.lengths[1])
+    assert n < 7 and (a.top_tokens[1, n:] == stop).all()
+    for x in (a.logprobs, a.entropy, a.top_logprobs):
+        assert not x[1, n:].any() and x[1, :n].all()
+    assert torch.equal(a.top_tokens[1, :n], free.top_tokens[1, :n])
+    with torch.no_grad():
+        model.text_norm.weight.fill_(float("nan"))    # scores that are NaN are not 0 times NaN behind the stop
+    dec = ReasoningDecoder(model, 3, 5, max_new=3, stop_token=0)
+    b = dec(images, text)
+    for i in range(3):
+        n = int(b.lengths[i])
+        assert b.logprobs[i, :n].isnan().all() and not b.logprobs[i, n:].any()
