@@ -111,7 +111,9 @@ class PagedKVCache:
     Every layer has pools [n_pages, page_size, Hkv, D]; one ``page_table`` [B, W] and one ``lengths``
     [B] (tokens stored so far) serve all layers. A forward pass over new tokens runs between
     ``begin(t, counts)`` and ``advance()``: in it each layer stores its t tokens (the first
-    ``counts[b]`` of them) behind ``lengths`` and attends over ``seen`` = lengths + stored tokens.
+    ``counts[b]`` of them) behind ``lengths`` and attends over ``seen`` = lengths + stored tokens. Several
+    tokens at once begin their sequences: ``begin`` refuses them once the cache holds tokens (until
+    ``reset``), because they would attend to one another alone.
     """
 
     def __init__(self, n_layers: int, batch_size: int, max_len: int, kv_heads: int, head_dim: int,
@@ -125,19 +127,24 @@ class PagedKVCache:
         self.seen = torch.zeros_like(self.lengths)
         self.max_len = max_len
         self.counts: torch.Tensor | None = None
+        self.begun = False  # whether tokens may be stored (known without reading the lengths back)
 
     def layer(self, i: int) -> "CacheLayer":
         return CacheLayer(self, i)
 
     def begin(self, tokens: int, counts: torch.Tensor | None = None) -> None:
+        if tokens > 1 and self.begun:
+            raise ValueError(f"the cache holds tokens already: {tokens} more have to enter one at a time")
         self.counts = counts
         torch.add(self.lengths, tokens if counts is None else counts, out=self.seen)
 
     def advance(self) -> None:
         self.lengths.copy_(self.seen)
+        self.begun = True
 
     def reset(self) -> None:
         self.lengths.zero_()
+        self.begun = False
 
 
 class CacheLayer:

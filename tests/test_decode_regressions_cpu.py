@@ -8,6 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig
+from nuvla_forge_b200.models.layers import PagedKVCache, run_blocks
 from nuvla_forge_b200.ops import logprobs as lp
 from nuvla_forge_b200.ops import paged
 from nuvla_forge_b200.serve import ReasoningDecoder
@@ -158,3 +159,26 @@ def test_every_score_behind_a_stop_token_is_zero():
     for i in range(3):
         n = int(b.lengths[i])
         assert b.logprobs[i, :n].isnan().all() and not b.logprobs[i, n:].any()
+
+
+@torch.no_grad()
+def test_several_tokens_do_not_enter_a_cache_that_holds_some():
+    """They would attend to one another alone; one at a time they see what is stored."""
+    model, _, _ = _model()
+    x = torch.randn(2, 6, 64)
+    whole = run_blocks(model.text_blocks, x, model.text_norm)
+    cache = PagedKVCache(2, 2, 8, 2, 16, page_size=4, dtype=torch.float32)
+
+    def feed(t0, t1):
+        cache.begin(t1 - t0)
+        h = run_blocks(model.text_blocks, x[:, t0:t1], model.text_norm, cache=cache)
+        cache.advance()
+        return h
+
+    for _ in range(2):
+        first = feed(0, 4)
+        with pytest.raises(ValueError, match="one at a time"):
+            feed(4, 6)
+        h = torch.cat([first, feed(4, 5), feed(5, 6)], 1)
+        assert (h - whole).abs().max() < TOL
+        cache.reset()
