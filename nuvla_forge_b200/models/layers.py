@@ -153,12 +153,13 @@ class CacheLayer:
     def __init__(self, cache: PagedKVCache, i: int):
         self.cache, self.k, self.v = cache, cache.k[i], cache.v[i]
 
-    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+    def append(self, k: torch.Tensor, v: torch.Tensor, force_reference: bool = False) -> None:
         c = self.cache
-        append_kv(k, v, self.k, self.v, c.page_table, c.lengths, c.counts)
+        append_kv(k, v, self.k, self.v, c.page_table, c.lengths, c.counts, force_reference=force_reference)
 
-    def attend(self, q: torch.Tensor) -> torch.Tensor:
-        return paged_attention(q, self.k, self.v, self.cache.page_table, self.cache.seen)
+    def attend(self, q: torch.Tensor, force_reference: bool = False) -> torch.Tensor:
+        return paged_attention(q, self.k, self.v, self.cache.page_table, self.cache.seen,
+                               force_reference=force_reference)
 
 
 class Attention(nn.Module):
@@ -206,9 +207,9 @@ class Attention(nn.Module):
                 kv = linear(context, self.qkv.weight[c:]).view(b, s, 2 * Hk, Dh)
             k, v = kv.split([Hk, Hk], dim=2)
         if cache is not None:
-            cache.append(k, v)
+            cache.append(k, v, force_reference=not self.fused)
         if cache is not None and t == 1:
-            o = cache.attend(q)
+            o = cache.attend(q, force_reference=not self.fused)
         else:
             o = attention_op(q, k, v, causal=self.causal and context is None, force_reference=not self.fused)
         o = o.reshape(b, t, c)

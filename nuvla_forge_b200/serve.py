@@ -19,7 +19,8 @@ the next token.
     waypoints = planner(answer.states)      # the DiT attends to the answer's states too
     waypoints = model.dit.sample(answer.context(b))   # or to one answer's, cut behind its stop token
 
-On CPU (or with ``graph=False``) both run the same code eagerly.
+On CPU (or with ``graph=False``) both run the same code eagerly; so does a ``ReasoningDecoder`` of a model
+with ``fused=False`` or without native kernels, whose reference operators read indices back.
 The reference has no inference path beyond ``TrajectoryDiT.sample``
 (nuvla_forge/model/dit.py:221-230, never called in its repository).
 """
@@ -31,6 +32,7 @@ from typing import NamedTuple
 
 import torch
 
+from . import _native as nat
 from .models.nuvla import NuVLA
 from .ops import paged, token_logprobs
 
@@ -136,7 +138,7 @@ class ReasoningDecoder:
         self.graph = None
         self._turn = threading.Lock()
         self._done: torch.cuda.Event | None = None   # the last use of the buffers above, on any stream
-        if graph and dev.type == "cuda":
+        if graph and dev.type == "cuda" and cfg.fused and nat.HAS_NATIVE and model.lm_head.dtype in nat.DT:
             with torch.cuda.device(dev):  # the capture is of the current device's stream
                 side = torch.cuda.Stream(dev)
                 side.wait_stream(torch.cuda.current_stream(dev))

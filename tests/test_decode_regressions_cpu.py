@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from nuvla_forge_b200.models import NuVLA, NuVLAConfig
+from nuvla_forge_b200.models import NuVLA, NuVLAConfig, layers
 from nuvla_forge_b200.models.layers import PagedKVCache, run_blocks
 from nuvla_forge_b200.ops import logprobs as lp
 from nuvla_forge_b200.ops import paged
@@ -182,3 +182,14 @@ def test_several_tokens_do_not_enter_a_cache_that_holds_some():
         h = torch.cat([first, feed(4, 5), feed(5, 6)], 1)
         assert (h - whole).abs().max() < TOL
         cache.reset()
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_decoding_honours_the_models_choice_of_kernels(fused, monkeypatch):
+    model, images, text = _model(fused=fused)
+    asked = []
+    for name in ("append_kv", "paged_attention"):
+        op = getattr(layers, name)
+        monkeypatch.setattr(layers, name, lambda *a, op=op, **kw: (asked.append(kw["force_reference"]), op(*a, **kw))[1])
+    ReasoningDecoder(model, 3, 5, max_new=2)(images, text)
+    assert len(asked) >= 6 and all(f is not fused for f in asked)

@@ -138,3 +138,21 @@ def test_forward_mode_derivatives_are_refused():
             paged.append_kv(dk, k, kc, kc.clone(), n.view(2, 1), n)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda z: lp.token_logprobs(z).entropy, (x,), (d,))
+
+
+def test_unfused_decoding_is_a_reference_of_its_own(monkeypatch):
+    """Plain operators decode, the kernels score what was decoded; fp32, tolerance as for the fused decoder."""
+    model, images, text = _model(torch.float32, text_heads=4, text_kv_heads=2)
+    plain = NuVLA(NuVLAConfig.preset("tiny", vocab_size=1000, n_instruction=8, n_reasoning=40, text_heads=4,
+                                     text_kv_heads=2, fused=False)).to(DEV)
+    plain.load_state_dict(model.state_dict())
+    call, names = nat.call, set()
+    monkeypatch.setattr(nat, "call", lambda name, *a: (names.add(name), call(name, *a))[1])
+    dec = ReasoningDecoder(plain, 4, 8, max_new=8, top_k=3, page_size=16)
+    a = dec(images, text)
+    assert dec.graph is None and not names & {"nfb_append_kv", "nfb_paged_attn", "nfb_logprobs_fwd"}
+    seq = torch.cat([text, a.tokens], 1)
+    with torch.no_grad():
+        s = model.score_text(images, seq[:, :-1], seq[:, 1:], top_k=3)
+    assert "nfb_logprobs_fwd" in names
+    assert (s.logprobs[:, 7:] - a.logprobs).abs().max() < 1e-2 and (s.entropy[:, 7:] - a.entropy).abs().max() < 1e-2
