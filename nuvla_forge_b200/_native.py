@@ -243,6 +243,16 @@ def on_device(device: torch.device):
     return torch.cuda.device(idx)
 
 
+def status_of(words: dict[int, torch.Tensor], device: torch.device | None) -> list[tuple[int, torch.Tensor]]:
+    """The (index, status word) pairs of ``words`` that a check of ``device`` (None: of all) is about."""
+    if device is None:
+        return sorted(words.items())
+    if device.type != "cuda":
+        return []
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    return [(idx, words[idx])] if idx in words else []
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt not in DT:
         raise TypeError(f"unsupported dtype {dt}")

@@ -40,8 +40,9 @@ def _status_word(device: torch.device) -> torch.Tensor:
 
 
 def check_status(device: torch.device | None = None) -> None:
-    """Raise if a kernel met a position, length or page id out of range (synchronises)."""
-    for idx, t in _status.items():
+    """Raise (and clear it) if a kernel met a position, length or page id out of range on ``device``, or on any without
+    one (synchronises)."""
+    for idx, t in nat.status_of(_status, device):
         v = int(t.item())
         if v:
             t.zero_()

@@ -193,3 +193,20 @@ def test_decoding_honours_the_models_choice_of_kernels(fused, monkeypatch):
         monkeypatch.setattr(layers, name, lambda *a, op=op, **kw: (asked.append(kw["force_reference"]), op(*a, **kw))[1])
     ReasoningDecoder(model, 3, 5, max_new=2)(images, text)
     assert len(asked) >= 6 and all(f is not fused for f in asked)
+
+
+@pytest.mark.parametrize("mod", [paged, lp])
+def test_check_status_is_about_the_device_it_is_given(mod):
+    bad = (3 << 24) | 1
+    mod._status.update({97: torch.tensor([bad], dtype=torch.int32), 98: torch.tensor([bad], dtype=torch.int32)})
+    try:
+        mod.check_status(torch.device("cpu"))
+        mod.check_status(torch.device("cuda", 96))
+        with pytest.raises(RuntimeError, match="cuda:98"):
+            mod.check_status(torch.device("cuda", 98))
+        mod.check_status(torch.device("cuda", 98))    # raising cleared it
+        with pytest.raises(RuntimeError, match="cuda:97"):
+            mod.check_status()                        # the other device's is still there
+        mod.check_status()
+    finally:
+        del mod._status[97], mod._status[98]
