@@ -41,8 +41,10 @@ def _status_word(device: torch.device) -> torch.Tensor:
 
 def check_status(device: torch.device | None = None) -> None:
     """Raise (and clear it) if a kernel met a position, length or page id out of range on ``device``, or on any without
-    one (synchronises)."""
+    one (waits for every stream of it)."""
     for idx, t in nat.status_of(_status, device):
+        if t.is_cuda:
+            torch.cuda.synchronize(t.device)
         v = int(t.item())
         if v:
             t.zero_()

@@ -156,3 +156,24 @@ def test_unfused_decoding_is_a_reference_of_its_own(monkeypatch):
         s = model.score_text(images, seq[:, :-1], seq[:, 1:], top_k=3)
     assert "nfb_logprobs_fwd" in names
     assert (s.logprobs[:, 7:] - a.logprobs).abs().max() < 1e-2 and (s.entropy[:, 7:] - a.entropy).abs().max() < 1e-2
+
+
+def test_check_status_waits_for_kernels_on_other_streams():
+    kc = torch.zeros(2, 16, 2, 64, device=DEV, dtype=torch.bfloat16)
+    table, n = torch.tensor([[5]], dtype=torch.int32, device=DEV), torch.tensor([3], dtype=torch.int32, device=DEV)
+    q = torch.zeros(1, 1, 2, 64, device=DEV, dtype=torch.bfloat16)
+    x, t = torch.zeros(2, 40, device=DEV), torch.tensor([3, 40], device=DEV)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        paged.paged_attention(q, kc, kc, table, n)    # a page id out of range: skipped and reported
+        lp.token_logprobs(x, t)
+    with pytest.raises(RuntimeError, match="out of range"):
+        paged.check_status()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        lp.token_logprobs(x, t)
+    with pytest.raises(RuntimeError, match="outside the vocabulary"):
+        lp.check_status()
+    paged.check_status()
