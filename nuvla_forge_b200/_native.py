@@ -243,6 +243,17 @@ def on_device(device: torch.device):
     return torch.cuda.device(idx)
 
 
+def status_word(words: dict[int, torch.Tensor], device: torch.device) -> torch.Tensor:
+    """The device's word of ``words``, created by the first call (an ordinary tensor, also under inference mode:
+    whoever reads it later has to be able to clear it)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    t = words.get(idx)
+    if t is None:
+        with torch.inference_mode(False):
+            t = words[idx] = torch.zeros(1, dtype=torch.int32, device=device)
+    return t
+
+
 def status_of(words: dict[int, torch.Tensor], device: torch.device | None) -> list[tuple[int, torch.Tensor]]:
     """The (index, status word) pairs of ``words`` that a check of ``device`` (None: of all) is about."""
     if device is None:

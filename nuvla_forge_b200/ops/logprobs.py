@@ -32,11 +32,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    t = _status.get(idx)
-    if t is None:
-        t = _status[idx] = torch.zeros(1, dtype=torch.int32, device=device)
-    return t
+    return nat.status_word(_status, device)
 
 
 def check_status(device: torch.device | None = None) -> None:

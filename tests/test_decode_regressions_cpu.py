@@ -7,6 +7,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from nuvla_forge_b200 import _native as nat
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig, layers
 from nuvla_forge_b200.models.layers import PagedKVCache, run_blocks
 from nuvla_forge_b200.ops import logprobs as lp
@@ -210,3 +211,17 @@ def test_check_status_is_about_the_device_it_is_given(mod):
         mod.check_status()
     finally:
         del mod._status[97], mod._status[98]
+
+
+@pytest.mark.parametrize("mod", [paged, lp])
+def test_a_status_word_made_under_inference_mode_can_be_cleared(mod):
+    with torch.inference_mode():
+        word = mod._status_word(torch.device("cpu", 99))
+        word.fill_((3 << 24) | 1)
+    try:
+        assert not word.is_inference()
+        with pytest.raises(RuntimeError, match="cuda:99"):
+            mod.check_status()
+        mod.check_status()
+    finally:
+        del mod._status[99]
