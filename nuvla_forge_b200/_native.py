@@ -238,19 +238,22 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.curre
 def on_device(device: torch.device):
     """Context in which ``device`` is current (kernels launch on the current device)."""
     idx = device.index
-    if idx is None or idx == _current_device():
+    if idx is None or device.type != "cuda" or idx == _current_device():
         return _NO_GUARD
     return torch.cuda.device(idx)
 
 
 def status_word(words: dict[int, torch.Tensor], device: torch.device) -> torch.Tensor:
     """The device's word of ``words``, created by the first call (an ordinary tensor, also under inference mode:
-    whoever reads it later has to be able to clear it)."""
+    whoever reads it later has to be able to clear it), and not in a capture, whose every replay would clear it."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = words.get(idx)
     if t is None:
-        with torch.inference_mode(False):
-            t = words[idx] = torch.zeros(1, dtype=torch.int32, device=device)
+        with on_device(device), torch.inference_mode(False):
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the first call on {device} makes its status word: make one outside of the capture")
+            t = torch.zeros(1, dtype=torch.int32, device=device)
+            words[idx] = t
     return t
 
 

@@ -177,3 +177,39 @@ def test_check_status_waits_for_kernels_on_other_streams():
     with pytest.raises(RuntimeError, match="outside the vocabulary"):
         lp.check_status()
     paged.check_status()
+
+
+@pytest.fixture
+def no_status_words():
+    kept = {m: dict(m._status) for m in (paged, lp)}
+    for m in kept:
+        m._status.clear()
+    yield
+    for m, words in kept.items():
+        m._status.clear()
+        m._status.update(words)
+
+
+def _small_calls():
+    kc = torch.zeros(2, 16, 2, 64, device=DEV, dtype=torch.bfloat16)
+    n = torch.tensor([3], dtype=torch.int32, device=DEV)
+    q = torch.zeros(1, 1, 2, 64, device=DEV, dtype=torch.bfloat16)
+    tables = [torch.tensor([[i]], dtype=torch.int32, device=DEV) for i in (0, 5)]
+    x, targets = torch.zeros(2, 40, device=DEV), [torch.tensor([3, i], device=DEV) for i in (4, 40)]
+    return [(lambda bad, t=t: paged.paged_attention(q, kc, kc, t[bad], n)) for t in (tables,)] + \
+        [lambda bad: lp.token_logprobs(x, targets[bad])]
+
+
+def test_a_first_call_in_a_capture_is_refused(no_status_words):
+    for call, mod in zip(_small_calls(), (paged, lp)):
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside of the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call(0)
+        assert not mod._status
+        call(0)                                       # outside of it, then in one
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(0)
+        g.replay()
+        mod.check_status()
