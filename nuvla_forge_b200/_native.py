@@ -245,7 +245,8 @@ def on_device(device: torch.device):
 
 def status_word(words: dict[int, torch.Tensor], device: torch.device) -> torch.Tensor:
     """The device's word of ``words``, created by the first call (an ordinary tensor, also under inference mode:
-    whoever reads it later has to be able to clear it), and not in a capture, whose every replay would clear it."""
+    whoever reads it later has to be able to clear it). It is finished before the call goes on, since later calls may
+    be on other streams, and not created in a capture, whose every replay would clear it."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = words.get(idx)
     if t is None:
@@ -253,6 +254,8 @@ def status_word(words: dict[int, torch.Tensor], device: torch.device) -> torch.T
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"the first call on {device} makes its status word: make one outside of the capture")
             t = torch.zeros(1, dtype=torch.int32, device=device)
+            if t.is_cuda:
+                torch.cuda.current_stream(device).synchronize()
             words[idx] = t
     return t
 

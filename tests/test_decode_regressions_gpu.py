@@ -213,3 +213,17 @@ def test_a_first_call_in_a_capture_is_refused(no_status_words):
             call(0)
         g.replay()
         mod.check_status()
+
+
+def test_an_error_on_another_stream_outlives_the_first_calls_status_word(no_status_words):
+    calls = _small_calls()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for call, mod in zip(calls, (paged, lp)):
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(50_000_000)
+            call(0)
+        with torch.cuda.stream(b):
+            call(1)
+        with pytest.raises(RuntimeError, match="out"):
+            mod.check_status()
