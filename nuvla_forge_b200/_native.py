@@ -92,7 +92,7 @@ _SIGS: dict[str, tuple] = {
     "nfb_gemm_swiglu_fwd": (I, [P, P, P, P, I, I, I, L, L, L, L, P, P]),
     "nfb_gemm_swiglu_bwd": (I, [P, P, P, P, I, I, I, L, L, L, L, P, P]),
     "nfb_append_kv": (I, [I, P, P, P, P, P, P, P, P, P, P, P, P, P, P]),
-    "nfb_paged_attn_ws": (L, [L, L, L, L, L]),
+    "nfb_paged_attn_ws": (L, [I, L, L, L, L, L]),
     "nfb_paged_attn": (I, [I, P, P, P, P, P, P, P, P, F, P, P]),
     "nfb_logprobs_fwd": (I, [I, P, L, L, L, P, L, I, P, P, P, P, P, P, P]),
     "nfb_logprobs_bwd": (I, [I, P, L, L, L, P, L, I, P, P, P, P, P, P, P, P]),

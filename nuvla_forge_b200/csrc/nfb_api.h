@@ -238,8 +238,10 @@ NFB_EXPORT int nfb_append_kv(int dtype, const void* q, const void* k, const void
                              void* v_cache, const int32_t* table, const int32_t* starts, const int32_t* counts,
                              const float* cos, const float* sin, const int64_t* dims, uint32_t* status,
                              void* stream);
-/* fp32 values of workspace that nfb_paged_attn needs (capacity = table_width * page_size). */
-NFB_EXPORT int64_t nfb_paged_attn_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity);
+/* fp32 values of workspace that nfb_paged_attn needs (capacity = table_width * page_size) with its tensor-core
+ * kernel (mma 1: 16-bit types, D 32, 64, 96 or 128, everything on 16 bytes) or its plain one (0); -1: the
+ * kernel cannot divide a call of this size. */
+NFB_EXPORT int64_t nfb_paged_attn_ws(int mma, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity);
 NFB_EXPORT int nfb_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_cache,
                               const int32_t* table, const int32_t* lengths, void* out, float* ws,
                               const int64_t* dims, float scale, uint32_t* status, void* stream);

@@ -1223,12 +1223,9 @@ NFB_API int nfb_append_kv(int dtype, const void* q, const void* k, const void* v
   return (int)cudaErrorInvalidValue;
 }
 
-NFB_API int64_t nfb_paged_attn_ws(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity) {
+NFB_API int64_t nfb_paged_attn_ws(int mma, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity) {
   AttnArgs a;
-  if (!plan(B, Hq, Hkv, D, capacity, false, nfb_num_sms(), a)) return -1;
-  const int64_t n = ws_floats(a);
-  if (!plan(B, Hq, Hkv, D, capacity, true, nfb_num_sms(), a)) return -1;
-  return n > ws_floats(a) ? n : ws_floats(a);
+  return plan(B, Hq, Hkv, D, capacity, mma != 0, nfb_num_sms(), a) ? ws_floats(a) : -1;
 }
 
 // dims: B, Hq, Hkv, D, page_size, n_pages, table_width, then the strides q (b, h), out (b, h),

@@ -192,17 +192,22 @@ def _attention_plan(key, q, k_cache, v_cache, page_table, lengths) -> tuple:
         raise ValueError(f"{Hkv} key heads do not divide {Hq} query heads")
     if not 0 < D <= MAX_HEAD_DIM:
         raise ValueError(f"head size {D} is not in 1..{MAX_HEAD_DIM}")
-    native, dims, ws = _native(q), None, 0
+    native, dims, ws, aligned = _native(q), None, 0, False
     if native and _rows_ok(q, page_table, lengths):
         n_pages, ps = k_cache.shape[:2]
         W = page_table.shape[1]
         dims = nat.int64s(B, Hq, Hkv, D, ps, n_pages, W, q.stride(0), q.stride(2), Hq * D, D, *k_cache.stride()[:3],
                           *v_cache.stride()[:3], page_table.stride(0))
-        ws = int(nat.lib().nfb_paged_attn_ws(B, Hq, Hkv, D, ps * W))
+        # which kernel runs is left to the addresses where the rest allows the tensor-core one: room for either
+        strides = (q.stride(0), q.stride(2), *k_cache.stride()[:3], *v_cache.stride()[:3])
+        tiled = q.element_size() == 2 and D in (32, 64, 96, 128) and all(n % 8 == 0 for n in strides)
+        plain, mma = (int(nat.lib().nfb_paged_attn_ws(kind, B, Hq, Hkv, D, ps * W)) if kind == 0 or tiled else -1
+                      for kind in (0, 1))
+        ws, aligned = max(plain, mma), plain < 0
         if ws < 0:
             raise ValueError(f"{B} sequences of up to {ps * W} tokens and {Hkv} key heads are more than the kernel's "
                              f"2^31 (sequence, head, 16-token tile) units: narrow the page table")
-    return _keep(key, (native, dims, ws, D ** -0.5))
+    return _keep(key, (native, dims, ws, aligned, D ** -0.5))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -218,7 +223,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     plan = _plans.get(key)
     if plan is None:
         plan = _attention_plan(key, q, k_cache, v_cache, page_table, lengths)
-    native, dims, n_ws, default = plan
+    native, dims, n_ws, aligned, default = plan
     if (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("paged_attention has no backward pass: call it under torch.no_grad()")
     if nat.has_tangent(q, k_cache, v_cache):
@@ -228,6 +233,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, sc)
     if dims is None:
         return paged_attention(_inner(q), k_cache, v_cache, _inner(page_table), _inner(lengths), sc)
+    if aligned and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("a page table as wide as this one needs queries and caches that begin on 16 bytes")
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     # the caching allocator's memory, new for each call and held until its kernels are launched: calls on other

@@ -82,7 +82,7 @@ def test_workspace_is_held_until_the_kernels_are_launched(monkeypatch):
     def between(name, *args):
         ws = args[7]
         assert name == "nfb_paged_attn" and ws is not None
-        n = int(nat.lib().nfb_paged_attn_ws(1, 8, 4, 64, 1600))
+        n = int(nat.lib().nfb_paged_attn_ws(1, 1, 8, 4, 64, 1600))
         other = [torch.empty(n, device=DEV) for _ in range(4)]       # of the workspace's size
         seen.append(all(not t.data_ptr() <= ws < t.data_ptr() + 4 * n for t in other))
         return call(name, *args)
@@ -227,3 +227,22 @@ def test_an_error_on_another_stream_outlives_the_first_calls_status_word(no_stat
             call(1)
         with pytest.raises(RuntimeError, match="out"):
             mod.check_status()
+
+
+def test_a_wide_table_is_refused_only_by_the_kernel_that_would_run():
+    """2^30 units of the tensor-core kernel, of 16 query heads each; the plain one counts 4 heads to a unit."""
+    g = torch.Generator(DEV).manual_seed(3)
+    kc, vc = (torch.randn(4, 16, 64, 64, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, 1, 1024, 64, generator=g, device=DEV).to(torch.bfloat16)
+    table, n = torch.tensor([[2, 0, 3]], dtype=torch.int32, device=DEV), torch.tensor([40], dtype=torch.int32, device=DEV)
+    wide = torch.zeros(1, 2 ** 24, dtype=torch.int32, device=DEV)
+    wide[:, :3] = table
+    want = paged.paged_attention(q, kc, vc, table, n)
+    out = paged.paged_attention(q, kc, vc, wide, n)   # the same function; another division adds in another order
+    assert torch.allclose(out.float(), want.float(), rtol=2 ** -7, atol=2 ** -9)
+    odd = torch.zeros(q.numel() + 1, device=DEV, dtype=torch.bfloat16)[1:].view(q.shape)
+    with pytest.raises(ValueError, match="16 bytes"):
+        paged.paged_attention(odd, kc, vc, wide, n)
+    with pytest.raises(ValueError, match="narrow the page table"):
+        paged.paged_attention(q.float(), kc.float(), vc.float(), wide, n)
+    paged.check_status()
