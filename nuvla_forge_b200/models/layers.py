@@ -136,7 +136,8 @@ class PagedKVCache:
         if tokens > 1 and self.begun:
             raise ValueError(f"the cache holds tokens already: {tokens} more have to enter one at a time")
         self.counts = counts
-        torch.add(self.lengths, tokens if counts is None else counts, out=self.seen)
+        # (a count outside 0..tokens stores none or all of them)
+        torch.add(self.lengths, tokens if counts is None else counts.clamp(0, tokens), out=self.seen)
 
     def advance(self) -> None:
         self.lengths.copy_(self.seen)

@@ -225,3 +225,13 @@ def test_a_status_word_made_under_inference_mode_can_be_cleared(mod):
         mod.check_status()
     finally:
         del mod._status[99]
+
+
+def test_a_cache_counts_the_tokens_that_are_stored():
+    """append_kv stores none for a negative count and all for one past the tokens."""
+    c = PagedKVCache(1, 3, 10, 1, 4, page_size=3, dtype=torch.float32)
+    c.begin(2, torch.tensor([5, -1, 1], dtype=torch.int32))
+    c.layer(0).append(torch.ones(3, 2, 1, 4), torch.ones(3, 2, 1, 4))
+    assert c.seen.tolist() == [2, 0, 1] and float(c.k[0].sum()) == 3 * 4
+    c.advance()
+    assert c.lengths.tolist() == [2, 0, 1]
