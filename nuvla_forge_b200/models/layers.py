@@ -118,6 +118,9 @@ class PagedKVCache:
 
     def __init__(self, n_layers: int, batch_size: int, max_len: int, kv_heads: int, head_dim: int,
                  page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cpu"):
+        if min(n_layers, batch_size, max_len, kv_heads, head_dim, page_size) < 1:
+            raise ValueError(f"a cache needs layers, sequences, tokens, heads and pages of at least 1, got {n_layers} layers, "
+                             f"{batch_size} x {max_len} tokens, {kv_heads} heads of {head_dim}, pages of {page_size}")
         per = -(-max_len // page_size)
         shape = (batch_size * per, page_size, kv_heads, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]
@@ -133,6 +136,8 @@ class PagedKVCache:
         return CacheLayer(self, i)
 
     def begin(self, tokens: int, counts: torch.Tensor | None = None) -> None:
+        if tokens > self.max_len:
+            raise ValueError(f"{tokens} tokens do not fit the cache's {self.max_len}")
         if tokens > 1 and self.begun:
             raise ValueError(f"the cache holds tokens already: {tokens} more have to enter one at a time")
         self.counts = counts

@@ -235,3 +235,17 @@ def test_a_cache_counts_the_tokens_that_are_stored():
     assert c.seen.tolist() == [2, 0, 1] and float(c.k[0].sum()) == 3 * 4
     c.advance()
     assert c.lengths.tolist() == [2, 0, 1]
+
+
+def test_cache_refuses_sizes_that_it_cannot_hold():
+    for bad in (dict(page_size=0), dict(page_size=-3), dict(max_len=0), dict(batch_size=0), dict(kv_heads=0)):
+        with pytest.raises(ValueError, match="at least 1"):
+            PagedKVCache(**{**dict(n_layers=1, batch_size=2, max_len=10, kv_heads=1, head_dim=4, page_size=3), **bad})
+    model, images, text = _model()
+    with pytest.raises(ValueError, match="at least 1"):
+        ReasoningDecoder(model, 3, 5, max_new=2, page_size=0)
+    cache = model.new_cache(3, 4, page_size=3)        # room in the last page behind max_len is not the cache's
+    with pytest.raises(ValueError, match="do not fit"):
+        model.read_prompt(images, text, cache)
+    with pytest.raises(ValueError, match="do not fit"):
+        cache.begin(5)
