@@ -195,7 +195,7 @@ class ReasoningDecoder:
         if text_tokens.shape != (self.batch_size, self.prompt_len):
             raise ValueError(f"decoder was built for instructions {(self.batch_size, self.prompt_len)}, got "
                              f"{tuple(text_tokens.shape)}")
-        with self._turn:
+        with self._turn, nat.on_device(self.token.device):  # (kernels launch on the current device)
             if self._done is None:
                 return self._answer(images, text_tokens)
             stream = torch.cuda.current_stream(self.token.device)

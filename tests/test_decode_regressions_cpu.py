@@ -1,5 +1,6 @@
 """Cached decoding and scores on the CPU: calls that once went wrong."""
 
+import contextlib
 import threading
 import time
 
@@ -249,3 +250,21 @@ def test_cache_refuses_sizes_that_it_cannot_hold():
         model.read_prompt(images, text, cache)
     with pytest.raises(ValueError, match="do not fit"):
         cache.begin(5)
+
+
+def test_a_call_runs_with_the_models_device_current(monkeypatch):
+    """The GEMMs launch on the current device; the constructor's warm-up and capture had it set."""
+    model, images, text = _model()
+    dec = ReasoningDecoder(model, 3, 5, max_new=2)
+    inside, seen, read = [], [], model.read_prompt
+
+    @contextlib.contextmanager
+    def on_device(device):
+        inside.append(device)
+        yield
+        inside.pop()
+
+    monkeypatch.setattr(nat, "on_device", on_device)
+    monkeypatch.setattr(model, "read_prompt", lambda *a: (seen.append(list(inside)), read(*a))[1])
+    dec(images, text)
+    assert seen == [[model.lm_head.device]]
