@@ -110,6 +110,7 @@ class ReasoningDecoder:
     no decoding path.
     """
 
+    @torch.inference_mode(False)  # buffers that calls in any mode can write
     def __init__(self, model: NuVLA, batch_size: int, prompt_len: int, max_new: int | None = None, top_k: int = 5,
                  page_size: int = 64, stop_token: int | None = None, graph: bool = True, warmup: int = 2):
         cfg = model.cfg

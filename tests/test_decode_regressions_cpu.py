@@ -268,3 +268,13 @@ def test_a_call_runs_with_the_models_device_current(monkeypatch):
     monkeypatch.setattr(model, "read_prompt", lambda *a: (seen.append(list(inside)), read(*a))[1])
     dec(images, text)
     assert seen == [[model.lm_head.device]]
+
+
+def test_a_decoder_built_under_inference_mode_answers_outside_of_it():
+    model, images, text = _model()
+    want = ReasoningDecoder(model, 3, 5, max_new=3)(images, text)
+    with torch.inference_mode():
+        dec = ReasoningDecoder(model, 3, 5, max_new=3)
+        inside = dec(images, text)
+    for a in (inside, dec(images, text)):
+        assert all(torch.equal(x, y) for x, y in zip(a, want))
