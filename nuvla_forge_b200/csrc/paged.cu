@@ -1224,6 +1224,7 @@ NFB_API int nfb_append_kv(int dtype, const void* q, const void* k, const void* v
 }
 
 NFB_API int64_t nfb_paged_attn_ws(int mma, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t capacity) {
+  if (B < 1 || Hq < 1 || Hkv < 1 || D < 1) return 0;  // nothing to launch (and a division by no heads below)
   AttnArgs a;
   return plan(B, Hq, Hkv, D, capacity, mma != 0, nfb_num_sms(), a) ? ws_floats(a) : -1;
 }

@@ -1,6 +1,8 @@
 """Cached decoding and scores on the CPU: calls that once went wrong."""
 
 import contextlib
+import subprocess
+import sys
 import threading
 import time
 
@@ -9,6 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from nuvla_forge_b200 import _native as nat
+from nuvla_forge_b200._build import lib_path
 from nuvla_forge_b200.models import NuVLA, NuVLAConfig, layers
 from nuvla_forge_b200.models.layers import PagedKVCache, run_blocks
 from nuvla_forge_b200.ops import logprobs as lp
@@ -278,3 +281,19 @@ def test_a_decoder_built_under_inference_mode_answers_outside_of_it():
         inside = dec(images, text)
     for a in (inside, dec(images, text)):
         assert all(torch.equal(x, y) for x, y in zip(a, want))
+
+
+def test_a_workspace_of_no_heads_is_asked_for_without_a_division_by_zero():
+    """In a process of its own: the division ended it."""
+    if not lib_path().exists():
+        pytest.skip("the native library is not built")
+    code = f"import ctypes; f = ctypes.CDLL({str(lib_path())!r}).nfb_paged_attn_ws"
+    code += """
+from ctypes import c_int, c_int64 as L
+f.restype, f.argtypes = L, [c_int] + [L] * 5
+print([f(kind, *args) for kind in (0, 1) for args in ((2, 0, 1, 64, 100), (0, 4, 2, 64, 100))])
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and r.stdout.strip() == "[0, 0, 0, 0]", (r.returncode, r.stderr[-500:])
+    kc, n = torch.randn(4, 4, 2, 8), torch.tensor([3, 4], dtype=torch.int32)
+    assert paged.paged_attention(torch.zeros(2, 1, 0, 8), kc, kc, n.view(2, 1) % 4, n).shape == (2, 1, 0, 8)

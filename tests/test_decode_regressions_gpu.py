@@ -246,3 +246,14 @@ def test_a_wide_table_is_refused_only_by_the_kernel_that_would_run():
     with pytest.raises(ValueError, match="narrow the page table"):
         paged.paged_attention(q.float(), kc.float(), vc.float(), wide, n)
     paged.check_status()
+
+
+def test_calls_without_query_heads():
+    kc, n = torch.zeros(4, 16, 2, 64, device=DEV, dtype=torch.bfloat16), torch.tensor([3, 4], dtype=torch.int32, device=DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        c, q = kc.to(dtype), torch.zeros(2, 1, 0, 64, device=DEV, dtype=dtype)
+        assert paged.paged_attention(q, c, c, n.view(2, 1) - 3, n).shape == (2, 1, 0, 64)
+        k = torch.ones(2, 1, 2, 64, device=DEV, dtype=dtype)
+        assert paged.append_kv(k, k, c, c.clone(), n.view(2, 1) - 3, n, q=q).shape == (2, 1, 0, 64)
+        assert torch.equal(c[0, 3], k[0, 0]) and torch.equal(c[1, 4], k[1, 0])
+    paged.check_status()
