@@ -97,7 +97,7 @@ class Answer(NamedTuple):
         """States [1, n, D] of sequence ``b`` up to and with its stop token (waits for its length). The DiT attends to
         every state that it is given, so a plan from these does not depend on ``max_new``, one from ``states`` does."""
         n = self.states.shape[1] - self.tokens.shape[1] + int(self.lengths[b])
-        return self.states[b:b + 1, :n]
+        return self.states[b, None, :n]
 
 
 class ReasoningDecoder:
@@ -105,9 +105,9 @@ class ReasoningDecoder:
 
     Built for a batch size, ``prompt_len`` instruction tokens and ``max_new`` answer tokens (at most
     the model's text positions together). ``stop_token`` ends a sequence: its later tokens repeat it and
-    score 0 (they are read like others, so that ``states`` are those of the returned tokens). A decoder works on one answer at a time: calls from several threads
-    or streams wait for one another (build a decoder for each to have them at once). The reference has
-    no decoding path.
+    score 0 (they are read like others, so that ``states`` are those of the returned tokens). A decoder
+    works on one answer at a time: calls from several threads or streams wait for one another (build a
+    decoder for each to have them at once). The reference has no decoding path.
     """
 
     @torch.inference_mode(False)  # buffers that calls in any mode can write

@@ -297,3 +297,11 @@ print([f(kind, *args) for kind in (0, 1) for args in ((2, 0, 1, 64, 100), (0, 4,
     assert r.returncode == 0 and r.stdout.strip() == "[0, 0, 0, 0]", (r.returncode, r.stderr[-500:])
     kc, n = torch.randn(4, 4, 2, 8), torch.tensor([3, 4], dtype=torch.int32)
     assert paged.paged_attention(torch.zeros(2, 1, 0, 8), kc, kc, n.view(2, 1) % 4, n).shape == (2, 1, 0, 8)
+
+
+def test_context_of_an_answer_counted_from_the_end():
+    model, images, text = _model()
+    a = ReasoningDecoder(model, 3, 5, max_new=3)(images, text)
+    assert torch.equal(a.context(-1), a.context(2)) and a.context(-1).shape == (1, a.states.shape[1], 64)
+    with pytest.raises(IndexError):
+        a.context(3)
