@@ -228,7 +228,8 @@ def int64s(*values: int):
 
 def has_tangent(*tensors) -> bool:
     """Whether a tensor carries a forward-mode derivative, which a kernel called past autograd would drop."""
-    return fwd_ad._current_level >= 0 and any(t is not None and fwd_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return fwd_ad._current_level >= 0 and any(t is not None and fwd_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors)
 
 
 _NO_GUARD = contextlib.nullcontext()

@@ -45,7 +45,7 @@ __device__ __forceinline__ float below_max(float z, float m) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z - m), "f"(-1e4f));
   return r;
 }
-__device__ __forceinline__ float exp_of(float d) {  // 2^-22 relative
+__device__ __forceinline__ float exp_of(float d) {  // relative: 2^-22 of ex2, |d| 2^-24 of the rounded product
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * kLog2e));
   return y;
@@ -142,7 +142,11 @@ __device__ __forceinline__ float kth_of_warp(float v, int k) {
 //
 // What bounds it: for 16-bit logits the HBM's rate leaves 11 issue slots of an SM for a warp's 32 values,
 // and the sums take 8 with one exponential among them. Without alternatives 16384 x 32000 bf16 take
-// 178 us (5.9 TB/s, 92% of the measured copy rate); with 5 the issue slots bind (84% busy): 229 us.
+// 178 us (5.9 TB/s, 92% of the measured copy rate) at 1965 MHz, 203 us once the power limit holds the SMs
+// near 1680 MHz; with 5 the issue slots bind (84% busy): 233 us. With many alternatives (1500 x 150001:
+// 91 us with none, 124 us with 20, 206 us with 32) the search for the bound and the notes bind, and for
+// rows of a few hundred logits (100000 x 300: 142 us, with 5 alternatives 285 us; the bytes take 9 us) the
+// block's fixed work, 5 us a row without and 10 us with alternatives.
 constexpr int kLpUnroll = 4, kLpAbove = 512, kLpEqual = 128;
 
 template <typename T, int NT>
@@ -458,6 +462,8 @@ struct LpBwdArgs {
 // logits are on their way. The given tokens' places are written
 // again by the first threads, each with its whole value (a token may be the target and an alternative),
 // rounded once.
+// Rows whose distance differs from V by no multiple of 16 bytes (logits cut from an odd padded vocabulary) are
+// read and written value by value: 8192 x 32000 bf16 646 us, against 161 us dense or cut from 32008.
 // 40 registers: 16384 x 32000 bf16 312 us; 32 and a spill 321 us, 48 320 us, 64 349 us (fewer CTAs).
 template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(NT, 1536 / NT) logprobs_bwd_kernel(const LpBwdArgs a) {
@@ -589,7 +595,10 @@ int launch_fwd_nt(LpArgs& a, cudaStream_t st) {
 // Threads a row: few for short rows and where many rows fill the GPU anyway (less waiting for one
 // another: 16384 x 32000 bf16 with 5 alternatives 229 us with 128, 266 us with 256; 20000 x 2000 fp16
 // 57 us with 64, 89 us with 128), many for few rows or long ones (64 x 32000 bf16: 7.6 us with 256, 8.2 us
-// with 128; 1500 x 150001 with 32 alternatives 213 us against 458 us).
+// with 128; 1500 x 150001 with 32 alternatives 211 us against 461 us, whose notes overflow).
+// Above 128 KB a row 256 threads cost little with few alternatives (4000 x 80001 bf16 with 5: 139 us, 134 us
+// with 128; 1000 x 150001 fp32 with none: 117 us, 107 us) and save much with many (the latter with 32:
+// 390 us, 1199 us).
 template <typename T>
 int launch_fwd(LpArgs& a, cudaStream_t st) {
   const int64_t bytes = a.V * (int64_t)sizeof(T);

@@ -119,8 +119,9 @@ class PagedKVCache:
     def __init__(self, n_layers: int, batch_size: int, max_len: int, kv_heads: int, head_dim: int,
                  page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cpu"):
         if min(n_layers, batch_size, max_len, kv_heads, head_dim, page_size) < 1:
-            raise ValueError(f"a cache needs layers, sequences, tokens, heads and pages of at least 1, got {n_layers} layers, "
-                             f"{batch_size} x {max_len} tokens, {kv_heads} heads of {head_dim}, pages of {page_size}")
+            raise ValueError(f"a cache needs layers, sequences, tokens, heads and pages of at least 1, got {n_layers} "
+                             f"layers, {batch_size} x {max_len} tokens, {kv_heads} heads of {head_dim}, pages of "
+                             f"{page_size}")
         per = -(-max_len // page_size)
         shape = (batch_size * per, page_size, kv_heads, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_layers)]

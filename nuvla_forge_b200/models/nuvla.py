@@ -337,7 +337,7 @@ class NuVLA(nn.Module):
         """Sample waypoints [B, horizon, traj_dim] by Euler integration of the DiT's velocity."""
         return self.dit.sample(self.context(images, text_tokens), steps=steps, z0=z0)
 
-    # -- answering with the reasoning head (BASELINE layout) ---------------
+    # -- answering with the reasoning head (causal backbone) ---------------
     def _needs_causal_backbone(self) -> None:
         if not self.cfg.backbone_over_images:
             raise ValueError("answering needs the causal backbone over images and text (backbone_over_images); the "

@@ -119,8 +119,11 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     same. A masked logit is -inf; a row of nothing else has log p -inf, entropy 0 and no gradient. A row
     with a NaN or +inf logit gives NaN (and unspecified alternatives). A target outside the vocabulary
     gives NaN and is reported by ``check_status`` (on the CPU it raises). Nothing waits for the host; a call
-    can be captured in a CUDA graph after a first one outside of it, its backward pass only while no
+    can be captured in a CUDA graph after a first one outside of it (refused before), its backward pass only while no
     eager autograd graph of the same leaves is alive (torch ties their gradients to that graph's stream).
+    Rows may begin anywhere; the backward pass is about four times faster where their distance is V plus a multiple
+    of 16 bytes (a vocabulary of V padded to V + 8 16-bit logits rather than to V + 3). Only the reference has
+    forward-mode derivatives.
     """
     if logits.dim() < 1 or not logits.is_floating_point():
         raise TypeError(f"logits must be a floating-point tensor [..., V], got {tuple(logits.shape)} {logits.dtype}")

@@ -9,8 +9,8 @@ Layout: pools ``[n_pages, page_size, Hkv, D]`` for keys and values (the projecti
 ``ops.attention``), ``page_table`` [B, W] int32 page ids, ``lengths`` [B] int32. Token p of sequence
 b is in page ``page_table[b, p // page_size]``, slot ``p % page_size``; any page size works. Lengths
 and page ids stay on the device: neither op waits for the host, both can be captured in a CUDA
-graph (after a first call outside of one, which creates the device's status word), and several
-streams can run them at once on caches of their own.
+graph (after a first call outside of one, which creates the device's status word; refused before),
+and several streams can run them at once on caches of their own.
 
 A position or page id out of range cannot be refused without reading it back: the kernels skip the
 token and set a status word that ``check_status`` (and the trainer's health monitor) raises on. On
@@ -217,7 +217,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     q [B, 1, Hq, D] (grouped queries: Hkv divides Hq, D <= 256); returns [B, 1, Hq, D]. ``scale``
     defaults to D ** -0.5. A sequence of length 0 answers zeros; what the pages hold behind a
-    sequence's length is never used. Statistics and sums are fp32, whatever the cache's type.
+    sequence's length is never used. Statistics and sums are fp32, whatever the cache's type; of a weight
+    p <= 1, 16 bits or more meet the values (fp16: all but 2^-20 p or 2^-39).
     """
     key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(page_table), _sig(lengths))
     plan = _plans.get(key)
